@@ -597,6 +597,74 @@ int tagan_narrow_linear_bwd(int64_t M, int32_t K, int32_t N, const float* x, int
                             int64_t lddy, float* dw, float* db, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions.  Each pair (a, b) of a head's first `rot` features is turned by t = position * inv_freq[pair]:
+ *   (a, b) -> scale * (a cos t - b sin t, a sin t + b cos t)
+ * pairs are features (i, i + rot/2), or (2i, 2i + 1) with interleaved; features from `rot` on pass unchanged.
+ * Angles are formed in fp64 (far positions), the turn in fp32.  inverse turns back: the gradient of the turn.
+ * q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] with token / head strides in elements and unit
+ * feature stride (heads or kv_heads 0: that tensor is absent); outputs may be the inputs.  head_dim <= 256.
+ * positions [tokens] of tagan_pos_type; inv_freq [rot / 2] fp64.  No workspace.
+ * ------------------------------------------------------------------------- */
+enum tagan_pos_type { TAGAN_POS_I32 = 0, TAGAN_POS_I64 = 1, TAGAN_POS_F32 = 2, TAGAN_POS_F64 = 3 };
+int tagan_rotary(int dtype, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t rot,
+                 const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                 const void* positions, int32_t pos_type, const double* inv_freq, float scale, int interleaved,
+                 int inverse, void* q_out, int64_t qo_tok, int64_t qo_head, void* k_out, int64_t ko_tok,
+                 int64_t ko_head, void* stream);
+/* New tokens of a cache: token i of sequence b has position lens[b] + i; q is turned into q_out, k is turned into and
+ * v moved to row lens[b] + i of the caches (strides: sequence, token, head).  Rows outside [0, capacity) are not
+ * written.  lens is read, not advanced.  Sequences must not share cache rows. */
+int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                        int32_t rot, const void* q, int64_t q_b, int64_t q_tok, int64_t q_head, const void* k,
+                        int64_t k_b, int64_t k_tok, int64_t k_head, const void* v, int64_t v_b, int64_t v_tok,
+                        int64_t v_head, const int32_t* lens, const double* inv_freq, float scale, int interleaved,
+                        void* q_out, int64_t qo_b, int64_t qo_tok, int64_t qo_head, void* k_cache, int64_t kc_b,
+                        int64_t kc_tok, int64_t kc_head, void* v_cache, int64_t vc_b, int64_t vc_tok, int64_t vc_head,
+                        int64_t capacity, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over packed sequences.  q / out [nq, heads, head_dim], k / v [nk, kv_heads, head_dim]; sequence b has
+ * queries [offsets_q[b], offsets_q[b+1]) and keys [offsets_k[b], offsets_k[b+1]) (device int32 [n_seq + 1],
+ * ascending; values are clamped to the token counts).  Query head h reads key head h / (heads / kv_heads).
+ *   out = softmax(scale q kᵀ over the visible keys) v
+ * causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key), so every query i < Lq - Lk sees none;
+ * a row without a visible key, or outside every sequence, gives zeros.
+ * head_dim: multiples of 8 up to 128; heads / kv_heads <= 512; scale > 0.  Pointers and strides (elements) on 16
+ * bytes, feature stride 1, token strides of head_dim to 2^22.
+ * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
+ * no key is seen.  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
+ * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
+ * gradients.  workspace: tagan_packed_attn_bwd_workspace bytes.
+ * ------------------------------------------------------------------------- */
+int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                          int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
+                          const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
+                          float* lse, void* stream);
+size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads);
+int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                          int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
+                          const int32_t* offsets_k, int causal, float scale, const void* out, int64_t o_tok,
+                          int64_t o_head, const float* lse, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
+                          int64_t dq_tok, int64_t dq_head, void* dk, int64_t dk_tok, int64_t dk_head, void* dv,
+                          int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of new tokens against a cache (the last of the cached rows are the new tokens' own): q / out
+ * [batch, new_len, heads, head_dim], caches [batch, capacity, kv_heads, head_dim] with strides (sequence, token,
+ * head); lens [batch] device int32 = cached rows of each sequence, the new ones included (clamped to [0, capacity]).
+ * Query i sees rows j < lens[b] - new_len + 1 + i; none: zeros.  Rows from lens[b] on are never used, whatever they
+ * hold.  The key axis is split over workgroups where rows are few and joined in a second launch (workspace:
+ * tagan_cached_attn_workspace bytes, a function of these arguments only).  Limits as tagan_packed_attn_fwd. */
+size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
+                                   int32_t head_dim);
+int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
+                      int32_t head_dim, const void* q, int64_t q_b, int64_t q_tok, int64_t q_head, const void* k_cache,
+                      int64_t k_b, int64_t k_tok, int64_t k_head, const void* v_cache, int64_t v_b, int64_t v_tok,
+                      int64_t v_head, const int32_t* lens, float scale, void* out, int64_t o_b, int64_t o_tok,
+                      int64_t o_head, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,6 @@ repository-root shim ``tagan_amd.py`` maps the hyphenated directory name).
 from .model import TAGAN  # noqa: F401
 from .utils.config import TAGANConfig  # noqa: F401
 from .utils.memory_bank import NodeMemoryBank  # noqa: F401
-from . import layers, kernels  # noqa: F401
+from . import layers, kernels, packed  # noqa: F401
 
 __version__ = "0.1.0"

@@ -1,0 +1,1070 @@
+// Attention over packed sequences (different lengths behind one another, grouped key heads, causal), its backward, and
+// the serving form against a cache.  For one sequence and one key head, with the group's G query heads packed as rows
+// r = token * G + g:
+//   S = scale Q Kᵀ over the visible keys (j <= token + Lk - Lq when causal), P = softmax(S), O = P V
+//   dV = Pᵀ dO, dP = dO Vᵀ, dS = P (dP - rowsum(dO O)), dQ = scale dS K, dK = scale dSᵀ Q  (sums over the group's rows)
+// One pass over the keys with a running maximum and sum (fp32); a row that sees no key gives zeros.  The backward makes
+// P again from the stored log-sum-exp: one kernel over row tiles for dQ, one over key tiles for dK and dV, no atomics,
+// every sum in a fixed order.
+//
+// Matrix cores: 32x32 tiles, bf16 products of 16 (v_mfma_f32_32x32x16_bf16) or fp32 products of 2, accumulated in
+// fp32.  A fragment is 8 contraction values of a lane: lane l holds row (or column) l % 32 and the values
+// 8 (l / 32) .. + 7 of a run of 16.  Scores are formed transposed (keys in the accumulator's registers, the row in the
+// lane), so a row's softmax statistics are one per lane and its reduction is in registers plus one half swap; the
+// accumulator's 8 registers of a run of 16 keys are, converted, the second product's operand without any exchange,
+// because a contraction may take its keys in any order as long as both operands do: value j of half h is key
+// 4 h + j % 4 + 8 (j / 4).  The other operand comes transposed out of LDS in that order (ds_read_tr16 for bf16).
+//
+// LDS tiles are filled by direct loads (buffer_load ... lds); the descriptor's bound makes rows behind the sequence
+// and features behind head_dim zeros.  16-byte chunks are swizzled within a row so that both the row reads (16 rows,
+// one chunk) and the transposed reads (4 rows, 64 bytes) touch all banks once.
+#include "common.cuh"
+
+namespace tagan {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+#define TAGAN_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// ------------------------------------------------------------------------------------------------ fragments
+template <typename T>
+struct Frag;
+template <>
+struct Frag<uint16_t> {
+    union {
+        bf16x8 v;
+        s16x4 h[2];
+        uint32_t u[4];
+    };
+    __device__ __forceinline__ void zero() { u[0] = u[1] = u[2] = u[3] = 0; }
+};
+template <>
+struct Frag<float> {
+    float v[8];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    }
+};
+
+__device__ __forceinline__ void mma(f32x16& c, const Frag<uint16_t>& a, const Frag<uint16_t>& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& c, const Frag<float>& a, const Frag<float>& b) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+}
+
+// eight accumulator registers as an operand (bf16: one rounding to nearest even of each probability or its gradient)
+__device__ __forceinline__ void from_acc(Frag<uint16_t>& f, const f32x16& c, int at) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.u[j] = f2bf2(c[at + 2 * j], c[at + 2 * j + 1]);
+}
+__device__ __forceinline__ void from_acc(Frag<float>& f, const f32x16& c, int at) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.v[j] = c[at + j];
+}
+
+__device__ __forceinline__ void load_frag(Frag<uint16_t>& f, const uint16_t* p) {
+    const uint4 u = *(const uint4*)p;
+    f.u[0] = u.x; f.u[1] = u.y; f.u[2] = u.z; f.u[3] = u.w;
+}
+__device__ __forceinline__ void load_frag(Frag<float>& f, const float* p) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w;
+    f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+}
+__device__ __forceinline__ float dot(const Frag<uint16_t>& a, const Frag<uint16_t>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        s = fmaf(__uint_as_float(a.u[j] << 16), __uint_as_float(b.u[j] << 16), s);
+        s = fmaf(__uint_as_float(a.u[j] & 0xffff0000u), __uint_as_float(b.u[j] & 0xffff0000u), s);
+    }
+    return s;
+}
+__device__ __forceinline__ float dot(const Frag<float>& a, const Frag<float>& b) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(a.v[j], b.v[j], s);
+    return s;
+}
+
+__device__ __forceinline__ void store4(uint16_t* p, float a, float b, float c, float d) {
+    *(uint2*)p = make_uint2(f2bf2(a, b), f2bf2(c, d));
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+    *(float4*)p = make_float4(a, b, c, d);
+}
+
+// ------------------------------------------------------------------------------------------------ LDS tiles
+// [rows][D] of T, chunk c of row r at chunk c ^ swz(r)
+template <typename T, int D>
+struct Tile {
+    static constexpr int E = 16 / (int)sizeof(T);      // elements of a chunk
+    static constexpr int CPR = D / E;                  // chunks of a row: 4 to 32
+    static constexpr int ROW = D * (int)sizeof(T);     // bytes of a row
+
+    __device__ static __forceinline__ int swz(int r) {
+        if constexpr (CPR == 4) return (r >> 2) & 3;
+        else if constexpr (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+
+    // rows [0, rows) of a tile from global rows `stride` bytes apart, `valid` of them and `bytes` of each there
+    template <int ROWS, int WAVES>
+    __device__ static __forceinline__ void fill(char* lds, const T* base, uint32_t stride, int valid, uint32_t bytes) {
+        const uint32_t records = valid > 0 ? (uint32_t)(valid - 1) * stride + bytes : 0u;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)records, 0x00027000);
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        constexpr int STEPS = ROWS * CPR / (64 * WAVES);
+        static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int first = (s * WAVES + wave) * 64;
+            const int ci = first + (threadIdx.x & 63);
+            const int r = ci / CPR;
+            const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
+            const uint32_t at = off < bytes ? (uint32_t)r * stride + off : 0x7ffffff0u;   // past the bound: zeros
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + first * 16), 16, (int)at, 0, 0, 0);
+        }
+    }
+    // the same of packed rows r0 + i = token * G + g; `tok` and `head` strides in bytes
+    template <int ROWS, int WAVES>
+    __device__ static __forceinline__ void fill_rows(char* lds, const T* base, uint32_t tok, uint32_t head, int rem,
+                                                     int G, uint32_t magic, int valid, uint32_t bytes) {
+        // the last valid row bounds the span whatever the order of the strides
+        const int lt = (int)(((uint32_t)(rem + valid - 1) * magic) >> 20);
+        const uint32_t span = valid > 0 ? (uint32_t)lt * tok + (uint32_t)(G - 1) * head + bytes : 0u;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)span, 0x00027000);
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        constexpr int STEPS = ROWS * CPR / (64 * WAVES);
+        static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int first = (s * WAVES + wave) * 64;
+            const int ci = first + (threadIdx.x & 63);
+            const int r = ci / CPR;
+            const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
+            const uint32_t x = (uint32_t)(rem + r), t = (x * magic) >> 20, g = x - t * (uint32_t)G;
+            const uint32_t at = (r < valid && off < bytes) ? t * tok + g * head + off : 0x7ffffff0u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + first * 16), 16, (int)at, 0, 0, 0);
+        }
+    }
+
+    // operand of rows `row0 + l % 32`, features 16 c + 8 (l / 32) .. + 7
+    __device__ static __forceinline__ void rows(Frag<T>& f, const char* lds, int row0, int c) {
+        const int l = threadIdx.x & 63, r = row0 + (l & 31), h = l >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const uint4 u = *(const uint4*)(lds + r * ROW + (((2 * c + h) ^ swz(r)) << 4));
+            f.u[0] = u.x; f.u[1] = u.y; f.u[2] = u.z; f.u[3] = u.w;
+        } else {
+            const float4 a = *(const float4*)(lds + r * ROW + (((4 * c + 2 * h) ^ swz(r)) << 4));
+            const float4 b = *(const float4*)(lds + r * ROW + (((4 * c + 2 * h + 1) ^ swz(r)) << 4));
+            f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w;
+            f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+        }
+    }
+    // transposed operand: features 32 db + l % 32, rows row0 + 4 h + j % 4 + 8 (j / 4)
+    __device__ static __forceinline__ void cols(Frag<T>& f, char* lds, int row0, int db) {
+        const int l = threadIdx.x & 63, h = l >> 5;
+        if constexpr (sizeof(T) == 2) {
+            // a lane addresses 4 features of one row; within 16 lanes the 4 x 16 block comes back transposed
+            const int s = l & 15, c = 32 * db + (l & 16) + 4 * (s & 3);
+            const int r = row0 + 4 * h + (s >> 2), r2 = r + 8;
+            char* a = lds + r * ROW + (((c >> 3) ^ swz(r)) << 4) + (c & 7) * 2;
+            char* b = lds + r2 * ROW + (((c >> 3) ^ swz(r2)) << 4) + (c & 7) * 2;
+            f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TAGAN_LDS(s16x4, a));
+            f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TAGAN_LDS(s16x4, b));
+        } else {
+            const int c = 32 * db + (l & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = row0 + 4 * h + (j & 3) + 8 * (j >> 2);
+                f.v[j] = *(const float*)(lds + r * ROW + (((c >> 2) ^ swz(r)) << 4) + (c & 3) * 4);
+            }
+        }
+    }
+};
+
+// Infinities and NaN among the values of a tile of which a row sees only a part: 0 * inf in a product would carry
+// them into rows that do not see them.  Such a tile is multiplied with finite values and with two masks instead.
+__device__ __forceinline__ bool wild(uint32_t u, uint16_t) {
+    return (u & 0x7f800000u) == 0x7f800000u || (u & 0x7f80u) == 0x7f80u;
+}
+__device__ __forceinline__ bool wild(uint32_t u, float) { return (u & 0x7f800000u) == 0x7f800000u; }
+template <typename T, int BYTES>
+__device__ __forceinline__ bool any_wild(const char* lds) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < BYTES / 1024; ++i) {
+        const uint4 u = *(const uint4*)(lds + i * 1024 + (threadIdx.x & 63) * 16);
+        bad |= wild(u.x, T()) || wild(u.y, T()) || wild(u.z, T()) || wild(u.w, T());
+    }
+    return __any(bad);
+}
+// f without its infinities and NaN; up / down: 1 where +inf / -inf was, both where NaN was
+__device__ __forceinline__ void tame(Frag<uint16_t>& f, Frag<uint16_t>& up, Frag<uint16_t>& down) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        up.u[j] = down.u[j] = 0;
+#pragma unroll
+        for (int x = 0; x < 32; x += 16) {
+            const uint32_t v = (f.u[j] >> x) & 0xffffu;
+            if ((v & 0x7f80u) != 0x7f80u) continue;
+            f.u[j] &= ~(0xffffu << x);
+            if (v != 0xff80u) up.u[j] |= 0x3f80u << x;
+            if (v != 0x7f80u) down.u[j] |= 0x3f80u << x;
+        }
+    }
+}
+__device__ __forceinline__ void tame(Frag<float>& f, Frag<float>& up, Frag<float>& down) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t v = __float_as_uint(f.v[j]);
+        const bool bad = (v & 0x7f800000u) == 0x7f800000u;
+        up.v[j] = bad && v != 0xff800000u ? 1.f : 0.f;
+        down.v[j] = bad && v != 0x7f800000u ? 1.f : 0.f;
+        if (bad) f.v[j] = 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void mma_tame(f32x16& c, Frag<T>& a, const Frag<T>& b) {
+    Frag<T> up, down;
+    tame(a, up, down);
+    mma(c, a, b);
+    f32x16 n;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n[i] = 0.f;
+    mma(n, up, b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (n[i] > 0.f) c[i] += INFINITY;
+        n[i] = 0.f;
+    }
+    mma(n, down, b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (n[i] > 0.f) c[i] -= INFINITY;
+}
+
+// every direct load of this wave has arrived, then of the workgroup
+__device__ __forceinline__ void tiles_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+__device__ __forceinline__ float half_max(float x) {
+    float a, b;
+    swap32(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    float a, b;
+    swap32(x, a, b);
+    return a + b;
+}
+
+// ------------------------------------------------------------------------------------------------ sequences
+struct Strides {
+    int64_t b, tok, head;   // elements
+};
+
+struct AttnArgs {
+    const void *q, *k, *v, *o, *dout;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta;
+    Strides qs, ks, vs, os, dos, dqs, dks, dvs;
+    const int32_t *offs_q, *offs_k;   // packed: [n_seq + 1]; null: a cache
+    const int32_t* lens;              // cache: [batch] keys of each
+    int64_t nq, nk;                   // packed: tokens in all; cache: new tokens and capacity of each
+    int32_t n_seq, heads, kv_heads, G, dim, causal, splits;
+    uint32_t magic;                   // (x * magic) >> 20 = x / G for x < G + 256 (G <= 512)
+    float c;                          // scale * log2(e)
+    float scale;
+    float* part;                      // splits: [split][row of batch][D + 4]
+};
+
+// One sequence and where its rows lie.  Rows outside every sequence belong to two more that see no key (the run before
+// the first offset and the run behind the last), so they get zeros.
+struct Seq {
+    int64_t q0, k0;    // first token, first key (elements of the token axis)
+    int32_t lq, lk, index;
+    int32_t tile;      // tile of this sequence
+};
+
+__device__ __forceinline__ int64_t edge(const int32_t* offs, int n_seq, int64_t n, int i) {
+    if (i == 0) return 0;
+    if (i == n_seq + 2) return n;
+    const int64_t e = offs[i - 1];
+    return e < 0 ? 0 : (e > n ? n : e);
+}
+
+// The sequence of virtual tile vt: sequence i starts at floor(edge_i * mul / tile) + i, which leaves each room for
+// ceil(length * mul / tile) tiles.  64 probes to a step of the search.
+__device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int64_t n, int mul, int tile, int64_t vt) {
+    int lo = 0, count = n_seq + 2;
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int i = lo + (int)(threadIdx.x & 63) * step;
+        const bool at = i < lo + count && edge(offs, n_seq, n, i) * mul / tile + i <= vt;
+        const int hit = __popcll(__ballot(at));
+        const int next = lo + (hit > 0 ? hit - 1 : 0) * step;
+        count = min(step, lo + count - next);
+        lo = next;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ __forceinline__ int64_t tile_of(const int32_t* offs, int n_seq, int64_t n, int mul, int tile, int64_t vt,
+                                           int i) {
+    return vt - (edge(offs, n_seq, n, i) * mul / tile + i);
+}
+
+// rows of a query tile: sequence, false where the tile is none
+template <int ROWS>
+__device__ __forceinline__ bool locate(const AttnArgs& A, int64_t vt, Seq& s) {
+    if (A.offs_q == nullptr) {
+        const int64_t tiles = (A.nq * A.G + ROWS - 1) / ROWS;
+        s.index = (int)(vt / tiles);
+        s.tile = (int)(vt - s.index * tiles);
+        s.lq = (int)A.nq;
+        s.q0 = s.k0 = 0;
+        const int n = A.lens[s.index];
+        s.lk = n < 0 ? 0 : (int)min((int64_t)n, A.nk);
+        return true;
+    }
+    const int i = find_seq(A.offs_q, A.n_seq, A.nq, A.G, ROWS, vt);
+    const int64_t t = tile_of(A.offs_q, A.n_seq, A.nq, A.G, ROWS, vt, i);
+    s.q0 = edge(A.offs_q, A.n_seq, A.nq, i);
+    const int64_t lq = edge(A.offs_q, A.n_seq, A.nq, i + 1) - s.q0;
+    if (lq <= 0 || t * ROWS >= lq * A.G) return false;
+    s.lq = (int)lq;
+    s.tile = (int)t;
+    s.index = 0;
+    s.k0 = 0;
+    s.lk = 0;
+    if (i >= 1 && i <= A.n_seq) {
+        s.k0 = edge(A.offs_k, A.n_seq, A.nk, i);
+        const int64_t lk = edge(A.offs_k, A.n_seq, A.nk, i + 1) - s.k0;
+        s.lk = lk < 0 ? 0 : (int)lk;
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename T, int D>
+struct Shape {
+    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB); 32 where fp32 doubles that
+    static constexpr int KT = sizeof(T) == 4 && D == 128 ? 32 : 64;
+};
+
+// A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
+template <typename T, int D, int WAVES, bool SPLIT>
+__global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
+    constexpr int KT = Shape<T, D>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    typedef Tile<T, D> TL;
+    __shared__ __align__(16) char ks[KT * TL::ROW];
+    __shared__ __align__(16) char vs[KT * TL::ROW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    int64_t bid = blockIdx.x;
+    int split = 0;
+    if constexpr (SPLIT) {
+        split = (int)(bid % A.splits);
+        bid /= A.splits;
+    }
+    const int hk = (int)(bid % A.kv_heads);
+    // last tiles first: with a causal mask they have the most keys
+    const int64_t tiles = (int64_t)gridDim.x / A.kv_heads / (SPLIT ? A.splits : 1);
+    Seq sq;
+    if (!locate<ROWS>(A, tiles - 1 - bid / A.kv_heads, sq)) return;
+
+    const int G = A.G;
+    const int64_t nrows = (int64_t)sq.lq * G;
+    const int64_t r0 = (int64_t)sq.tile * ROWS;
+    const int64_t row = r0 + wave * 32 + (lane & 31);
+    const bool mine = row < nrows;
+    const int token = (int)(row / G), g = (int)(row - (int64_t)token * G);
+    const int past = sq.lk - sq.lq;       // keys before the first query's own
+    // keys that this lane's row, and that the whole block, can see
+    const int see = !mine ? 0 : (A.causal ? min(sq.lk, max(0, token + past + 1)) : sq.lk);
+    const int last_tok = (int)((min(r0 + ROWS, nrows) - 1) / G);
+    int kend = A.causal ? min(sq.lk, max(0, last_tok + past + 1)) : sq.lk;
+    int kbeg = 0;
+    if constexpr (SPLIT) {
+        const int per = ((kend + A.splits - 1) / A.splits + KT - 1) / KT * KT;
+        kbeg = min(kend, split * per);
+        kend = min(kend, kbeg + per);
+    }
+    // the least and the most that a row of this wave sees: whole tiles before the least need no mask
+    const int64_t w0 = r0 + wave * 32;
+    const int first_tok = (int)(w0 / G);
+    const int wave_least = w0 + 31 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, first_tok + past + 1)) : sq.lk);
+    const int wave_last = w0 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, (int)((min(w0 + 32, nrows) - 1) / G) + past + 1)) : sq.lk);
+
+    const T* Q = (const T*)A.q + (int64_t)sq.index * A.qs.b + (sq.q0 + token) * A.qs.tok + (int64_t)(hk * G + g) * A.qs.head;
+    const T* K = (const T*)A.k + (int64_t)sq.index * A.ks.b + sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + (int64_t)sq.index * A.vs.b + sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
+    const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
+
+    Frag<T> qf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        qf[c].zero();
+        if (mine && 16 * c + 8 * half < A.dim) load_frag(qf[c], Q + 16 * c + 8 * half);
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    for (int kt = kbeg; kt < kend; kt += KT) {
+        __syncthreads();
+        const int valid = min(KT, kend - kt);
+        TL::template fill<KT, WAVES>(ks, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(vs, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+        tiles_ready();
+        if (kt >= wave_last) continue;
+        f32x16 s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                Frag<T> kf;
+                TL::rows(kf, ks, 32 * b, c);
+                mma(s[b], kf, qf[c]);
+            }
+        }
+        const bool masked = kt + KT > wave_least || kt + KT > kend;
+        if (masked) {
+            const int lim = min(see, kend) - kt - 4 * half;   // keys of this lane below it are visible
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[b][i] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = fmaxf(m, half_max(top));
+        const float base = top == -INFINITY ? 0.f : top * A.c;
+        const float alpha = __builtin_amdgcn_exp2f(m * A.c - base);   // m = -inf: 0
+        m = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], A.c, -base));
+                sum += s[b][i];
+            }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        if (masked && any_wild<T, KT * TL::ROW>(vs)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    Frag<T> pf;
+                    from_acc(pf, s[b], 8 * x);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        Frag<T> vf;
+                        TL::cols(vf, vs, 32 * b + 16 * x, d);
+                        mma_tame(o[d], vf, pf);
+                    }
+                }
+            continue;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                Frag<T> pf;
+                from_acc(pf, s[b], 8 * x);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> vf;
+                    TL::cols(vf, vs, 32 * b + 16 * x, d);
+                    mma(o[d], vf, pf);
+                }
+            }
+    }
+    l = half_sum(l);
+    if (!mine) return;
+    if constexpr (SPLIT) {
+        // unnormalised sums with their maximum (in powers of two) and total
+        float* p = A.part + (((int64_t)split * A.n_seq + sq.index) * A.kv_heads + hk) * nrows * (D + 4) + row * (D + 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                store4(p + 32 * d + 2 * i + 4 * half, o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+        if (half == 0) *(float2*)(p + D) = make_float2(m * A.c, l);
+    } else {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        T* O = (T*)A.out + (int64_t)sq.index * A.os.b + (sq.q0 + token) * A.os.tok + (int64_t)(hk * G + g) * A.os.head;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int at = 32 * d + 2 * i + 4 * half;
+                if (at < A.dim)
+                    store4(O + at, o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv);
+            }
+        // +inf where no key is seen: exp2(s - lse) is 0 in the backward
+        if (A.lse && half == 0)
+            A.lse[(sq.q0 + token) * A.heads + hk * G + g] = l == 0.f ? INFINITY : m * A.c + __log2f(l);
+    }
+}
+
+// joins the splits of a row: 32 lanes to a row, D / 32 features to a lane
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
+    constexpr int E = D / 32;
+    const int64_t rows = A.nq * A.G, all = (int64_t)A.n_seq * A.kv_heads * rows;
+    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= all) return;
+    const int x = threadIdx.x & 31;
+    const int64_t bh = at / rows, row = at - bh * rows;
+    const float* p = A.part + at * (D + 4);
+    const int64_t step = all * (D + 4);
+    float m = -INFINITY;
+    for (int s = 0; s < A.splits; ++s) {
+        const float2 ml = *(const float2*)(p + s * step + D);
+        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    }
+    float l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int s = 0; s < A.splits; ++s) {
+        const float2 ml = *(const float2*)(p + s * step + D);
+        if (ml.y == 0.f) continue;
+        const float w = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(ml.y, w, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(p[s * step + x * E + e], w, o[e]);
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const int64_t b = bh / A.kv_heads, token = row / A.G;
+    const int head = (int)(bh - b * A.kv_heads) * A.G + (int)(row - token * A.G);
+    T* out = (T*)A.out + b * A.os.b + token * A.os.tok + (int64_t)head * A.os.head;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (x * E + e < A.dim) {
+            if constexpr (sizeof(T) == 4) out[x * E + e] = o[e] * inv;
+            else out[x * E + e] = (uint16_t)f2bf2(o[e] * inv, 0.f);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ
+// Rows as in the forward; also writes delta = rowsum(dO O) for the key kernel that follows on the stream.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
+    constexpr int KT = Shape<T, D>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    typedef Tile<T, D> TL;
+    __shared__ __align__(16) char ks[KT * TL::ROW];
+    __shared__ __align__(16) char vs[KT * TL::ROW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int hk = (int)(blockIdx.x % A.kv_heads);
+    const int64_t tiles = gridDim.x / A.kv_heads;
+    Seq sq;
+    if (!locate<ROWS>(A, tiles - 1 - blockIdx.x / A.kv_heads, sq)) return;
+    const int G = A.G;
+    const int64_t nrows = (int64_t)sq.lq * G;
+    const int64_t r0 = (int64_t)sq.tile * ROWS;
+    const int64_t row = r0 + wave * 32 + (lane & 31);
+    const bool mine = row < nrows;
+    const int token = (int)(row / G), g = (int)(row - (int64_t)token * G);
+    const int past = sq.lk - sq.lq;
+    const int see = !mine ? 0 : (A.causal ? min(sq.lk, max(0, token + past + 1)) : sq.lk);
+    const int last_tok = (int)((min(r0 + ROWS, nrows) - 1) / G);
+    const int kend = A.causal ? min(sq.lk, max(0, last_tok + past + 1)) : sq.lk;
+    const int64_t w0 = r0 + wave * 32;
+    const int first_tok = (int)(w0 / G);
+    const int wave_least = w0 + 31 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, first_tok + past + 1)) : sq.lk);
+    const int wave_last = w0 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, (int)((min(w0 + 32, nrows) - 1) / G) + past + 1)) : sq.lk);
+
+    const int64_t head = hk * G + g, tok = sq.q0 + token;
+    const T* Q = (const T*)A.q + tok * A.qs.tok + head * A.qs.head;
+    const T* O = (const T*)A.o + tok * A.os.tok + head * A.os.head;
+    const T* DO = (const T*)A.dout + tok * A.dos.tok + head * A.dos.head;
+    const T* K = (const T*)A.k + sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
+    const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
+
+    Frag<T> qf[NC], gf[NC];
+    float delta = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        qf[c].zero();
+        gf[c].zero();
+        if (mine && 16 * c + 8 * half < A.dim) {
+            Frag<T> of;
+            load_frag(qf[c], Q + 16 * c + 8 * half);
+            load_frag(gf[c], DO + 16 * c + 8 * half);
+            load_frag(of, O + 16 * c + 8 * half);
+            delta += dot(gf[c], of);
+        }
+    }
+    delta = half_sum(delta);
+    float lse = INFINITY;
+    if (mine) {
+        lse = A.lse[tok * A.heads + head];
+        if (half == 0) A.delta[tok * A.heads + head] = delta;
+    }
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
+
+    for (int kt = 0; kt < kend; kt += KT) {
+        __syncthreads();
+        const int valid = min(KT, kend - kt);
+        TL::template fill<KT, WAVES>(ks, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(vs, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+        tiles_ready();
+        if (kt >= wave_last) continue;
+        const bool masked = kt + KT > wave_least;
+        const int lim = see - kt - 4 * half;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                Frag<T> kf, vf;
+                TL::rows(kf, ks, 32 * b, c);
+                mma(s, kf, qf[c]);
+                TL::rows(vf, vs, 32 * b, c);
+                mma(dp, vf, gf[c]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -lse));
+                s[i] = p * (dp[i] - delta);
+            }
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (32 * b + 8 * (i >> 2) + (i & 3) >= lim) s[i] = 0.f;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                Frag<T> pf;
+                from_acc(pf, s, 8 * x);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> kf;
+                    TL::cols(kf, ks, 32 * b + 16 * x, d);
+                    mma(dq[d], kf, pf);
+                }
+            }
+        }
+    }
+    if (!mine) return;
+    T* DQ = (T*)A.dq + tok * A.dqs.tok + head * A.dqs.head;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int at = 32 * d + 2 * i + 4 * half;
+            if (at < A.dim)
+                store4(DQ + at, dq[d][i] * A.scale, dq[d][i + 1] * A.scale, dq[d][i + 2] * A.scale,
+                       dq[d][i + 3] * A.scale);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+// A wave has 32 keys (in its lanes) and passes over the rows that see them, QT at a time for the whole block.
+template <typename T, int D, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) k_attn_dkv(AttnArgs A) {
+    typedef Tile<T, D> TL;
+    // rows of a tile: 32, or 64 where 32 would leave lanes of the direct loads without a chunk
+    constexpr int QT = TL::ROW >= 128 ? 32 : 64, NC = D / 16, ND = D / 32, KEYS = 32 * WAVES;
+    __shared__ __align__(16) char qs[QT * TL::ROW];
+    __shared__ __align__(16) char gs[QT * TL::ROW];
+    __shared__ __align__(16) float st[2][QT];          // log-sum-exp and delta of the rows
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int hk = (int)(blockIdx.x % A.kv_heads);
+    const int64_t vt = blockIdx.x / A.kv_heads;        // first keys first: with a causal mask most rows see them
+    const int i = find_seq(A.offs_k, A.n_seq, A.nk, 1, KEYS, vt);
+    const int64_t tile = tile_of(A.offs_k, A.n_seq, A.nk, 1, KEYS, vt, i);
+    const int64_t k0 = edge(A.offs_k, A.n_seq, A.nk, i);
+    const int64_t lk64 = edge(A.offs_k, A.n_seq, A.nk, i + 1) - k0;
+    if (lk64 <= 0 || tile * KEYS >= lk64) return;
+    const int lk = (int)lk64;
+    int64_t q0 = 0;
+    int lq = 0;
+    if (i >= 1 && i <= A.n_seq) {
+        q0 = edge(A.offs_q, A.n_seq, A.nq, i);
+        lq = (int)max((int64_t)0, edge(A.offs_q, A.n_seq, A.nq, i + 1) - q0);
+    }
+    const int G = A.G, past = lk - lq;
+    const int key0 = (int)tile * KEYS, key = key0 + wave * 32 + (lane & 31);
+    const bool mine = key < lk;
+    const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
+    const T* K = (const T*)A.k + (k0 + key) * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + (k0 + key) * A.vs.tok + (int64_t)hk * A.vs.head;
+    Frag<T> kf[NC], vf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        kf[c].zero();
+        vf[c].zero();
+        if (mine && 16 * c + 8 * half < A.dim) {
+            load_frag(kf[c], K + 16 * c + 8 * half);
+            load_frag(vf[c], V + 16 * c + 8 * half);
+        }
+    }
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) dk[d][x] = dv[d][x] = 0.f;
+
+    const int64_t nrows = (int64_t)lq * G;
+    // the first row that sees the block's first key
+    const int64_t rbeg = A.causal ? (int64_t)max(0, key0 - past) * G : 0;
+    for (int64_t r0 = rbeg; r0 < nrows; r0 += QT) {
+        const int t0 = (int)(r0 / G), rem = (int)(r0 - (int64_t)t0 * G);
+        const int valid = (int)min((int64_t)QT, nrows - r0);
+        const int64_t tok = q0 + t0;
+        __syncthreads();
+        TL::template fill_rows<QT, WAVES>(qs, (const T*)A.q + tok * A.qs.tok + (int64_t)hk * G * A.qs.head,
+                                          (uint32_t)(A.qs.tok * sizeof(T)), (uint32_t)(A.qs.head * sizeof(T)), rem, G,
+                                          A.magic, valid, bytes);
+        TL::template fill_rows<QT, WAVES>(gs, (const T*)A.dout + tok * A.dos.tok + (int64_t)hk * G * A.dos.head,
+                                          (uint32_t)(A.dos.tok * sizeof(T)), (uint32_t)(A.dos.head * sizeof(T)), rem, G,
+                                          A.magic, valid, bytes);
+        if ((int)threadIdx.x < QT) {
+            const int r = threadIdx.x;
+            const uint32_t x = (uint32_t)(rem + r), t = (x * A.magic) >> 20, g = x - t * (uint32_t)G;
+            const int64_t at = (tok + t) * A.heads + (int64_t)hk * G + g;
+            st[0][r] = r < valid ? A.lse[at] : INFINITY;
+            st[1][r] = r < valid ? A.delta[at] : 0.f;
+        }
+        tiles_ready();
+        // rows from `first` on (in local tokens) see this lane's key
+        const bool masked = A.causal && key0 + wave * 32 + 31 > t0 + past;
+#pragma unroll
+        for (int q = 0; q < QT; q += 32) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                Frag<T> f;
+                TL::rows(f, qs, q, c);
+                mma(s, f, kf[c]);
+                TL::rows(f, gs, q, c);
+                mma(dp, f, vf[c]);
+            }
+            const int lim = masked ? (key - past - t0) * G - rem - q - 4 * half : -1;   // rows of this lane below it do not see
+#pragma unroll
+            for (int x = 0; x < 16; x += 4) {
+                const float4 ls = *(const float4*)&st[0][q + 2 * x + 4 * half];
+                const float4 de = *(const float4*)&st[1][q + 2 * x + 4 * half];
+                const float lx[4] = {ls.x, ls.y, ls.z, ls.w}, dx[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const bool ok = mine && 2 * x + y >= lim;
+                    const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[x + y], A.c, -lx[y])) : 0.f;
+                    s[x + y] = p;
+                    dp[x + y] = ok ? p * (dp[x + y] - dx[y]) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                Frag<T> pf, sf;
+                from_acc(pf, s, 8 * x);
+                from_acc(sf, dp, 8 * x);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> f;
+                    TL::cols(f, gs, q + 16 * x, d);
+                    mma(dv[d], f, pf);
+                    TL::cols(f, qs, q + 16 * x, d);
+                    mma(dk[d], f, sf);
+                }
+            }
+        }
+    }
+    if (!mine) return;
+    T* DK = (T*)A.dk + (k0 + key) * A.dks.tok + (int64_t)hk * A.dks.head;
+    T* DV = (T*)A.dv + (k0 + key) * A.dvs.tok + (int64_t)hk * A.dvs.head;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; x += 4) {
+            const int at = 32 * d + 2 * x + 4 * half;
+            if (at < A.dim) {
+                store4(DK + at, dk[d][x] * A.scale, dk[d][x + 1] * A.scale, dk[d][x + 2] * A.scale,
+                       dk[d][x + 3] * A.scale);
+                store4(DV + at, dv[d][x], dv[d][x + 1], dv[d][x + 2], dv[d][x + 3]);
+            }
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+constexpr int MAX_DIM = 128, MAX_GROUP = 512;
+
+bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int es) {
+    return !((uintptr_t)p & 15) && (a * es) % 16 == 0 && (b * es) % 16 == 0 && (c * es) % 16 == 0;
+}
+
+int check_shape(const char* what, int dtype, int64_t heads, int64_t kv_heads, int32_t dim, float scale) {
+    TAGAN_REQUIRE(dtype == TAGAN_F32 || dtype == TAGAN_BF16, TAGAN_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+    TAGAN_REQUIRE(kv_heads >= 1 && heads >= kv_heads && heads % kv_heads == 0 && heads / kv_heads <= MAX_GROUP,
+                  TAGAN_ERR_ARG, "%s: %lld heads over %lld key heads (a multiple, up to %d)", what, (long long)heads,
+                  (long long)kv_heads, MAX_GROUP);
+    TAGAN_REQUIRE(dim >= 8 && dim <= MAX_DIM && dim % 8 == 0, TAGAN_ERR_UNSUPPORTED,
+                  "%s: head_dim %d (a multiple of 8 up to %d)", what, dim, MAX_DIM);
+    TAGAN_REQUIRE(isfinite(scale) && scale > 0.f, TAGAN_ERR_ARG, "%s: scale has to be positive and finite", what);
+    return TAGAN_OK;
+}
+
+// strides that a tile's 32-bit offsets and 16-byte loads can take; tiled: read through buffer descriptors
+int check_tensor(const char* what, const char* name, const void* p, const Strides& s, int32_t dim, int es) {
+    TAGAN_REQUIRE(p, TAGAN_ERR_ARG, "%s: %s is null", what, name);
+    TAGAN_REQUIRE(aligned(p, s.b, s.tok, s.head, es), TAGAN_ERR_ARG,
+                  "%s: %s has to lie on 16 bytes, its strides too", what, name);
+    TAGAN_REQUIRE(s.tok >= dim && s.tok <= (1 << 22) && s.head >= 0 && s.head <= (1ll << 40) && s.b >= 0, TAGAN_ERR_ARG,
+                  "%s: %s has token stride %lld, head stride %lld", what, name, (long long)s.tok, (long long)s.head);
+    return TAGAN_OK;
+}
+
+uint32_t magic_of(int G) { return ((1u << 20) + (uint32_t)G - 1) / (uint32_t)G; }
+
+#define TAGAN_BY_DIM(T, dim, F)                                    \
+    ((dim) <= 32 ? F<T, 32> : (dim) <= 64 ? F<T, 64> : F<T, 128>)
+
+template <typename T, int D>
+int run_fwd(const AttnArgs& A, hipStream_t s) {
+    // waves to a block by the rows that a sequence has on average: 32-row blocks where four waves would mostly idle
+    const bool one = A.nq * A.G < (int64_t)64 * A.n_seq;
+    const int rows = one ? 32 : 128;
+    const int64_t blocks = (A.nq * A.G / rows + A.n_seq + 2) * A.kv_heads;
+    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
+    if (one) k_attn_fwd<T, D, 1, false><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, false><<<(unsigned)blocks, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("packed_attn_fwd");
+    return TAGAN_OK;
+}
+
+template <typename T, int D>
+int run_bwd(const AttnArgs& A, hipStream_t s) {
+    const bool one = A.nq * A.G < (int64_t)64 * A.n_seq, kone = A.nk < (int64_t)64 * A.n_seq;
+    const int64_t blocks = (A.nq * A.G / (one ? 32 : 128) + A.n_seq + 2) * A.kv_heads;
+    const int64_t kblocks = (A.nk / (kone ? 32 : 128) + A.n_seq + 2) * A.kv_heads;
+    TAGAN_REQUIRE(blocks <= 0x7fffffff && kblocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED,
+                  "packed_attn_bwd: too many tiles");
+    if (A.nq > 0) {
+        if (one) k_attn_dq<T, D, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+        else k_attn_dq<T, D, 4><<<(unsigned)blocks, 256, 0, s>>>(A);
+        TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
+    }
+    if (A.nk > 0) {
+        if (kone) k_attn_dkv<T, D, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
+        else k_attn_dkv<T, D, 4><<<(unsigned)kblocks, 256, 0, s>>>(A);
+        TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
+    }
+    return TAGAN_OK;
+}
+
+// Splits of the key axis for a cache: enough one-wave blocks for 8 to a CU, and at least 128 keys of the capacity to
+// each (the lengths themselves are on the device; a split divides the length it finds there)
+int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity, bool one) {
+    const int64_t blocks = batch * kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128));
+    const int64_t want = ((one ? 2048 : 512) + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t most = (capacity + 127) / 128;
+    const int64_t n = want < most ? want : most;
+    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+bool cache_one(int64_t rows) { return rows < 64; }
+
+template <typename T, int D>
+int run_cached(const AttnArgs& A, hipStream_t s) {
+    const int64_t rows = A.nq * A.G;
+    const bool one = cache_one(rows);
+    const int64_t blocks = (int64_t)A.n_seq * A.kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128)) * A.splits;
+    const int64_t joins = ((int64_t)A.n_seq * A.kv_heads * rows + 7) / 8;
+    TAGAN_REQUIRE(blocks <= 0x7fffffff && joins <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
+    if (A.splits == 1) {
+        if (one) k_attn_fwd<T, D, 1, false><<<(unsigned)blocks, 64, 0, s>>>(A);
+        else k_attn_fwd<T, D, 4, false><<<(unsigned)blocks, 256, 0, s>>>(A);
+        TAGAN_CHECK_LAUNCH("cached_attn");
+        return TAGAN_OK;
+    }
+    if (one) k_attn_fwd<T, D, 1, true><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, true><<<(unsigned)blocks, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("cached_attn");
+    k_attn_join<T, D><<<(unsigned)joins, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("cached_attn (join)");
+    return TAGAN_OK;
+}
+
+int padded_dim(int32_t dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+}  // namespace
+}  // namespace tagan
+
+using namespace tagan;
+
+extern "C" {
+
+int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                          int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
+                          const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
+                          float* lse, void* stream) {
+    int rc = check_shape("packed_attn_fwd", dtype, heads, kv_heads, head_dim, scale);
+    if (rc != TAGAN_OK) return rc;
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
+                  "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    if (nq == 0) return TAGAN_OK;
+    TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_fwd: null offsets");
+    const int es = dtype == TAGAN_F32 ? 4 : 2;
+    AttnArgs A = {};
+    A.q = q; A.k = k; A.v = v; A.out = out; A.lse = lse;
+    A.qs = {0, q_tok, q_head};
+    A.ks = {0, k_tok, k_head};
+    A.vs = {0, v_tok, v_head};
+    A.os = {0, o_tok, o_head};
+    if ((rc = check_tensor("packed_attn_fwd", "q", q, A.qs, head_dim, es)) != TAGAN_OK) return rc;
+    if (nk > 0) {
+        if ((rc = check_tensor("packed_attn_fwd", "k", k, A.ks, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("packed_attn_fwd", "v", v, A.vs, head_dim, es)) != TAGAN_OK) return rc;
+    }
+    if ((rc = check_tensor("packed_attn_fwd", "out", out, A.os, head_dim, es)) != TAGAN_OK) return rc;
+    A.offs_q = offsets_q; A.offs_k = offsets_k;
+    A.nq = nq; A.nk = nk; A.n_seq = n_seq;
+    A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
+    A.causal = causal != 0; A.splits = 1;
+    A.magic = magic_of(A.G);
+    A.scale = scale; A.c = scale * LOG2E;
+    hipStream_t s = as_stream(stream);
+    return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_fwd)(A, s)
+                              : TAGAN_BY_DIM(uint16_t, head_dim, run_fwd)(A, s);
+}
+
+size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads) {
+    return nq > 0 && heads > 0 ? (size_t)nq * (size_t)heads * 4 : 0;
+}
+
+int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                          int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
+                          const int32_t* offsets_k, int causal, float scale, const void* out, int64_t o_tok,
+                          int64_t o_head, const float* lse, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
+                          int64_t dq_tok, int64_t dq_head, void* dk, int64_t dk_tok, int64_t dk_head, void* dv,
+                          int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_shape("packed_attn_bwd", dtype, heads, kv_heads, head_dim, scale);
+    if (rc != TAGAN_OK) return rc;
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
+                  "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    if (nq == 0 && nk == 0) return TAGAN_OK;
+    TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_bwd: null offsets");
+    TAGAN_REQUIRE(workspace_bytes >= tagan_packed_attn_bwd_workspace(nq, heads) && (nq == 0 || (workspace && lse)),
+                  TAGAN_ERR_WORKSPACE, "packed_attn_bwd: workspace of %zu bytes", workspace_bytes);
+    const int es = dtype == TAGAN_F32 ? 4 : 2;
+    AttnArgs A = {};
+    A.q = q; A.k = k; A.v = v; A.o = out; A.dout = dout;
+    A.dq = dq; A.dk = dk; A.dv = dv;
+    A.lse = (float*)lse; A.delta = (float*)workspace;
+    A.qs = {0, q_tok, q_head};
+    A.ks = {0, k_tok, k_head};
+    A.vs = {0, v_tok, v_head};
+    A.os = {0, o_tok, o_head};
+    A.dos = {0, do_tok, do_head};
+    A.dqs = {0, dq_tok, dq_head};
+    A.dks = {0, dk_tok, dk_head};
+    A.dvs = {0, dv_tok, dv_head};
+    const struct { const char* name; const void* p; const Strides& s; int64_t n; } all[] = {
+        {"q", q, A.qs, nq}, {"out", out, A.os, nq}, {"dout", dout, A.dos, nq}, {"dq", dq, A.dqs, nq},
+        {"k", k, A.ks, nk}, {"v", v, A.vs, nk}, {"dk", dk, A.dks, nk}, {"dv", dv, A.dvs, nk}};
+    for (const auto& x : all)
+        if (x.n > 0 && (rc = check_tensor("packed_attn_bwd", x.name, x.p, x.s, head_dim, es)) != TAGAN_OK) return rc;
+    A.offs_q = offsets_q; A.offs_k = offsets_k;
+    A.nq = nq; A.nk = nk; A.n_seq = n_seq;
+    A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
+    A.causal = causal != 0; A.splits = 1;
+    A.magic = magic_of(A.G);
+    A.scale = scale; A.c = scale * LOG2E;
+    // a tile of packed rows spans (32 / G + 2) tokens and G heads in 31 bits
+    TAGAN_REQUIRE((q_head > do_head ? q_head : do_head) * A.G * es < (1ll << 30), TAGAN_ERR_UNSUPPORTED,
+                  "packed_attn_bwd: head strides %lld and %lld", (long long)q_head, (long long)do_head);
+    hipStream_t s = as_stream(stream);
+    return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_bwd)(A, s)
+                              : TAGAN_BY_DIM(uint16_t, head_dim, run_bwd)(A, s);
+}
+
+size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
+                                   int32_t head_dim) {
+    if (batch <= 0 || new_len <= 0 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
+    const int64_t rows = (int64_t)new_len * (heads / kv_heads);
+    const int n = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
+    return n == 1 ? 0 : (size_t)n * (size_t)batch * (size_t)(kv_heads * rows) * (size_t)(padded_dim(head_dim) + 4) * 4;
+}
+
+int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
+                      int32_t head_dim, const void* q, int64_t q_b, int64_t q_tok, int64_t q_head, const void* k_cache,
+                      int64_t k_b, int64_t k_tok, int64_t k_head, const void* v_cache, int64_t v_b, int64_t v_tok,
+                      int64_t v_head, const int32_t* lens, float scale, void* out, int64_t o_b, int64_t o_tok,
+                      int64_t o_head, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_shape("cached_attn", dtype, heads, kv_heads, head_dim, scale);
+    if (rc != TAGAN_OK) return rc;
+    TAGAN_REQUIRE(batch >= 0 && batch <= 0x7fffffff && new_len >= 0 && capacity >= 0 && capacity <= 0x7fffffff,
+                  TAGAN_ERR_ARG, "cached_attn: batch %lld new_len %d capacity %lld", (long long)batch, new_len,
+                  (long long)capacity);
+    if (batch == 0 || new_len == 0) return TAGAN_OK;
+    TAGAN_REQUIRE(lens, TAGAN_ERR_ARG, "cached_attn: null lens");
+    const int es = dtype == TAGAN_F32 ? 4 : 2;
+    AttnArgs A = {};
+    A.q = q; A.k = k_cache; A.v = v_cache; A.out = out;
+    A.qs = {q_b, q_tok, q_head};
+    A.ks = {k_b, k_tok, k_head};
+    A.vs = {v_b, v_tok, v_head};
+    A.os = {o_b, o_tok, o_head};
+    if ((rc = check_tensor("cached_attn", "q", q, A.qs, head_dim, es)) != TAGAN_OK) return rc;
+    if (capacity > 0) {
+        if ((rc = check_tensor("cached_attn", "k_cache", k_cache, A.ks, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("cached_attn", "v_cache", v_cache, A.vs, head_dim, es)) != TAGAN_OK) return rc;
+    }
+    if ((rc = check_tensor("cached_attn", "out", out, A.os, head_dim, es)) != TAGAN_OK) return rc;
+    A.lens = lens;
+    A.nq = new_len; A.nk = capacity; A.n_seq = (int32_t)batch;
+    A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
+    A.causal = 1;
+    A.magic = magic_of(A.G);
+    A.scale = scale; A.c = scale * LOG2E;
+    const int64_t rows = (int64_t)new_len * A.G;
+    A.splits = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
+    A.part = (float*)workspace;
+    const size_t need = tagan_cached_attn_workspace(batch, new_len, capacity, heads, kv_heads, head_dim);
+    TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), TAGAN_ERR_WORKSPACE,
+                  "cached_attn: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+    hipStream_t s = as_stream(stream);
+    return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_cached)(A, s)
+                              : TAGAN_BY_DIM(uint16_t, head_dim, run_cached)(A, s);
+}
+
+}  // extern "C"
