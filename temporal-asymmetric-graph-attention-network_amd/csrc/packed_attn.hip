@@ -32,6 +32,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 #define TAGAN_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
 
 constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LAZY = 8.f;
 
 // ------------------------------------------------------------------------------------------------ fragments
 template <typename T>
@@ -194,66 +195,34 @@ struct Tile {
     }
 };
 
-// Infinities and NaN among the values of a tile of which a row sees only a part: 0 * inf in a product would carry
-// them into rows that do not see them.  Such a tile is multiplied with finite values and with two masks instead.
-__device__ __forceinline__ bool wild(uint32_t u, uint16_t) {
-    return (u & 0x7f800000u) == 0x7f800000u || (u & 0x7f80u) == 0x7f80u;
+// Infinities and NaN among the values of a tile of which some row sees only a part: 0 * inf in the product would carry
+// them into rows that do not see them.  Such a tile is multiplied with zeros in their place, and after the last tile
+// each row adds those that it does see (any weight times an infinity is that infinity).
+__device__ __forceinline__ bool wild(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+template <typename T>
+__device__ __forceinline__ bool tame(uint32_t& w) {
+    const uint32_t was = w;
+    if (wild(__uint_as_float(w))) w = sizeof(T) == 2 ? w & 0x0000ffffu : 0u;
+    if (sizeof(T) == 2 && wild(__uint_as_float(w << 16))) w &= 0xffff0000u;
+    return w != was;
 }
-__device__ __forceinline__ bool wild(uint32_t u, float) { return (u & 0x7f800000u) == 0x7f800000u; }
-template <typename T, int BYTES>
-__device__ __forceinline__ bool any_wild(const char* lds) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < BYTES / 1024; ++i) {
-        const uint4 u = *(const uint4*)(lds + i * 1024 + (threadIdx.x & 63) * 16);
-        bad |= wild(u.x, T()) || wild(u.y, T()) || wild(u.z, T()) || wild(u.w, T());
-    }
-    return __any(bad);
-}
-// f without its infinities and NaN; up / down: 1 where +inf / -inf was, both where NaN was
-__device__ __forceinline__ void tame(Frag<uint16_t>& f, Frag<uint16_t>& up, Frag<uint16_t>& down) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        up.u[j] = down.u[j] = 0;
-#pragma unroll
-        for (int x = 0; x < 32; x += 16) {
-            const uint32_t v = (f.u[j] >> x) & 0xffffu;
-            if ((v & 0x7f80u) != 0x7f80u) continue;
-            f.u[j] &= ~(0xffffu << x);
-            if (v != 0xff80u) up.u[j] |= 0x3f80u << x;
-            if (v != 0x7f80u) down.u[j] |= 0x3f80u << x;
+// the whole workgroup: whether a tile had any, and zeros in their place
+template <typename T, int BYTES, int WAVES>
+__device__ __forceinline__ bool tame_tile(char* lds) {
+    bool any = false;
+#pragma unroll 1
+    for (int at = threadIdx.x * 16; at < BYTES; at += WAVES * 1024) {
+        uint4 u = *(const uint4*)(lds + at);
+        const bool x = tame<T>(u.x), y = tame<T>(u.y), z = tame<T>(u.z), w = tame<T>(u.w);
+        if (x || y || z || w) {
+            *(uint4*)(lds + at) = u;
+            any = true;
         }
     }
+    return __syncthreads_or(any) != 0;
 }
-__device__ __forceinline__ void tame(Frag<float>& f, Frag<float>& up, Frag<float>& down) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t v = __float_as_uint(f.v[j]);
-        const bool bad = (v & 0x7f800000u) == 0x7f800000u;
-        up.v[j] = bad && v != 0xff800000u ? 1.f : 0.f;
-        down.v[j] = bad && v != 0x7f800000u ? 1.f : 0.f;
-        if (bad) f.v[j] = 0.f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void mma_tame(f32x16& c, Frag<T>& a, const Frag<T>& b) {
-    Frag<T> up, down;
-    tame(a, up, down);
-    mma(c, a, b);
-    f32x16 n;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) n[i] = 0.f;
-    mma(n, up, b);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        if (n[i] > 0.f) c[i] += INFINITY;
-        n[i] = 0.f;
-    }
-    mma(n, down, b);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (n[i] > 0.f) c[i] -= INFINITY;
-}
+__device__ __forceinline__ float as_float(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ float as_float(float v) { return v; }
 
 // every direct load of this wave has arrived, then of the workgroup
 __device__ __forceinline__ void tiles_ready() {
@@ -360,19 +329,21 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int64_t vt, Seq& s) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int D>
+template <typename T, int D, int WAVES>
 struct Shape {
-    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB); 32 where fp32 doubles that
-    static constexpr int KT = sizeof(T) == 4 && D == 128 ? 32 : 64;
+    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB); 32 where fp32 doubles that, and for the widest heads of
+    // one-wave blocks, of which five then share a CU's LDS with two tiles each
+    static constexpr int KT = D == 128 && (sizeof(T) == 4 || WAVES == 1) ? 32 : 64;
 };
 
 // A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
 template <typename T, int D, int WAVES, bool SPLIT>
-__global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
-    constexpr int KT = Shape<T, D>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_fwd(AttnArgs A) {
+    constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
-    __shared__ __align__(16) char ks[KT * TL::ROW];
-    __shared__ __align__(16) char vs[KT * TL::ROW];
+    // two buffers, each an object of its own: reads of one do not wait for the loads of the other
+    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[KT * TL::ROW];
+    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[KT * TL::ROW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     int64_t bid = blockIdx.x;
     int split = 0;
@@ -403,6 +374,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
         kbeg = min(kend, split * per);
         kend = min(kend, kbeg + per);
     }
+    const int block_least = A.causal ? min(sq.lk, max(0, (int)(r0 / G) + past + 1)) : sq.lk;
     // the least and the most that a row of this wave sees: whole tiles before the least need no mask
     const int64_t w0 = r0 + wave * 32;
     const int first_tok = (int)(w0 / G);
@@ -425,15 +397,17 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, base = 0.f, l = 0.f;   // largest score of the base, that in powers of two, sum over it
 
-    for (int kt = kbeg; kt < kend; kt += KT) {
-        __syncthreads();
+    int wild_from = 0x7fffffff;                // first key of the tiles that were tamed
+    const auto load = [&](char* kb, char* vb, int kt) {
         const int valid = min(KT, kend - kt);
-        TL::template fill<KT, WAVES>(ks, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
-        TL::template fill<KT, WAVES>(vs, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
-        tiles_ready();
-        if (kt >= wave_last) continue;
+        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+    };
+    const auto tile = [&](char* ks, char* vs, int kt) {
+        if (min(kt + KT, kend) > block_least && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
+        if (kt >= wave_last) return;
         f32x16 s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -460,10 +434,22 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-        top = fmaxf(m, half_max(top));
-        const float base = top == -INFINITY ? 0.f : top * A.c;
-        const float alpha = __builtin_amdgcn_exp2f(m * A.c - base);   // m = -inf: 0
-        m = top;
+        top = half_max(top);
+        // The base of the exponents follows the maximum only where that has grown by more than LAZY powers of two
+        // (or had none): weights up to 2^LAZY lose nothing in fp32 sums and bf16 operands, and most tiles then
+        // leave the D / 2 output registers alone.
+        if (__any(top * A.c > base + LAZY || (m == -INFINITY && top > -INFINITY))) {
+            const float next = fmaxf(m, top);
+            const float b2 = next == -INFINITY ? 0.f : next * A.c;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base - b2);
+            m = next;
+            base = b2;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -472,27 +458,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
                 s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], A.c, -base));
                 sum += s[b][i];
             }
-        l = l * alpha + sum;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-        if (masked && any_wild<T, KT * TL::ROW>(vs)) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    Frag<T> pf;
-                    from_acc(pf, s[b], 8 * x);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        Frag<T> vf;
-                        TL::cols(vf, vs, 32 * b + 16 * x, d);
-                        mma_tame(o[d], vf, pf);
-                    }
-                }
-            continue;
-        }
+        l += sum;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -506,6 +472,29 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
                     mma(o[d], vf, pf);
                 }
             }
+    };
+    if (kbeg < kend) load(ks0, vs0, kbeg);
+    for (int kt = kbeg; kt < kend; kt += 2 * KT) {
+        tiles_ready();                                  // and every wave is done with the other buffer
+        if (kt + KT < kend) load(ks1, vs1, kt + KT);
+        tile(ks0, vs0, kt);
+        if (kt + KT >= kend) break;
+        tiles_ready();
+        if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
+        tile(ks1, vs1, kt + KT);
+    }
+#pragma unroll 1
+    for (int key = wild_from; key < kend; ++key) {
+        const T* value = V + (int64_t)key * A.vs.tok;
+        const bool seen = key < see;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int at = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+                const float x = seen && at < A.dim ? as_float(value[at]) : 0.f;
+                if (wild(x)) o[d][i] += x;
+            }
     }
     l = half_sum(l);
     if (!mine) return;
@@ -517,7 +506,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 store4(p + 32 * d + 2 * i + 4 * half, o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
-        if (half == 0) *(float2*)(p + D) = make_float2(m * A.c, l);
+        if (half == 0) *(float2*)(p + D) = make_float2(base, l);
     } else {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         T* O = (T*)A.out + (int64_t)sq.index * A.os.b + (sq.q0 + token) * A.os.tok + (int64_t)(hk * G + g) * A.os.head;
@@ -531,54 +520,69 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_fwd(AttnArgs A) {
             }
         // +inf where no key is seen: exp2(s - lse) is 0 in the backward
         if (A.lse && half == 0)
-            A.lse[(sq.q0 + token) * A.heads + hk * G + g] = l == 0.f ? INFINITY : m * A.c + __log2f(l);
+            A.lse[(sq.q0 + token) * A.heads + hk * G + g] = l == 0.f ? INFINITY : base + __log2f(l);
     }
 }
 
-// joins the splits of a row: 32 lanes to a row, D / 32 features to a lane
+// Joins the splits of a row, a workgroup to a row: the weights of all splits first, then the sums, with the splits dealt
+// out to JG groups of D / 4 lanes whose partial sums are added in order.  At 256 splits a thread has 8 to 32 independent
+// loads instead of a chain of 256.
+constexpr int MAX_SPLITS = 256;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
-    constexpr int E = D / 32;
-    const int64_t rows = A.nq * A.G, all = (int64_t)A.n_seq * A.kv_heads * rows;
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= all) return;
-    const int x = threadIdx.x & 31;
-    const int64_t bh = at / rows, row = at - bh * rows;
+    constexpr int L = D / 4, JG = 256 / L;
+    __shared__ float w[MAX_SPLITS], red[4], tot[4];
+    __shared__ float4 sums[JG][L];
+    const int64_t rows = A.nq * A.G, all = (int64_t)A.n_seq * A.kv_heads * rows, at = blockIdx.x;
+    const int64_t bh = at / rows, row = at - bh * rows, step = all * (D + 4);
     const float* p = A.part + at * (D + 4);
-    const int64_t step = all * (D + 4);
-    float m = -INFINITY;
-    for (int s = 0; s < A.splits; ++s) {
-        const float2 ml = *(const float2*)(p + s * step + D);
-        if (ml.y != 0.f) m = fmaxf(m, ml.x);
+    const int s = threadIdx.x, wave = s >> 6;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s < A.splits) ml = *(const float2*)(p + s * step + D);
+    const bool some = ml.y != 0.f;             // a split without a visible key has no base
+    const float m = lane_max<64>(some ? ml.x : -INFINITY);
+    if ((s & 63) == 0) red[wave] = m;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float x = some ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
+    w[s] = x;
+    const float t = lane_sum<64>(some ? x * ml.y : 0.f);
+    if ((s & 63) == 0) tot[wave] = t;
+    __syncthreads();
+    const float l = (tot[0] + tot[1]) + (tot[2] + tot[3]);
+    const int f = s % L, g = s / L;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = g; i < A.splits; i += JG) {
+        const float4 v = *(const float4*)(p + i * step + 4 * f);
+        const float wi = w[i];
+        if (wi != 0.f) {                       // NaN weights too
+            o.x = fmaf(v.x, wi, o.x);
+            o.y = fmaf(v.y, wi, o.y);
+            o.z = fmaf(v.z, wi, o.z);
+            o.w = fmaf(v.w, wi, o.w);
+        }
     }
-    float l = 0.f, o[E];
+    sums[g][f] = o;
+    __syncthreads();
+    if (g != 0 || 4 * f >= A.dim) return;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int s = 0; s < A.splits; ++s) {
-        const float2 ml = *(const float2*)(p + s * step + D);
-        if (ml.y == 0.f) continue;
-        const float w = __builtin_amdgcn_exp2f(ml.x - m);
-        l = fmaf(ml.y, w, l);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(p[s * step + x * E + e], w, o[e]);
+    for (int i = 1; i < JG; ++i) {
+        const float4 v = sums[i][f];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const int64_t b = bh / A.kv_heads, token = row / A.G;
     const int head = (int)(bh - b * A.kv_heads) * A.G + (int)(row - token * A.G);
     T* out = (T*)A.out + b * A.os.b + token * A.os.tok + (int64_t)head * A.os.head;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (x * E + e < A.dim) {
-            if constexpr (sizeof(T) == 4) out[x * E + e] = o[e] * inv;
-            else out[x * E + e] = (uint16_t)f2bf2(o[e] * inv, 0.f);
-        }
+    store4(out + 4 * f, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ
 // Rows as in the forward; also writes delta = rowsum(dO O) for the key kernel that follows on the stream.
 template <typename T, int D, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
-    constexpr int KT = Shape<T, D>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     __shared__ __align__(16) char ks[KT * TL::ROW];
     __shared__ __align__(16) char vs[KT * TL::ROW];
@@ -894,10 +898,10 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
 // each (the lengths themselves are on the device; a split divides the length it finds there)
 int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity, bool one) {
     const int64_t blocks = batch * kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128));
-    const int64_t want = ((one ? 2048 : 512) + blocks - 1) / (blocks > 0 ? blocks : 1);
+    const int64_t want = ((one ? 4096 : 1024) + blocks - 1) / (blocks > 0 ? blocks : 1);
     const int64_t most = (capacity + 127) / 128;
     const int64_t n = want < most ? want : most;
-    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+    return (int)(n < 1 ? 1 : n > MAX_SPLITS ? MAX_SPLITS : n);
 }
 bool cache_one(int64_t rows) { return rows < 64; }
 
@@ -906,7 +910,7 @@ int run_cached(const AttnArgs& A, hipStream_t s) {
     const int64_t rows = A.nq * A.G;
     const bool one = cache_one(rows);
     const int64_t blocks = (int64_t)A.n_seq * A.kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128)) * A.splits;
-    const int64_t joins = ((int64_t)A.n_seq * A.kv_heads * rows + 7) / 8;
+    const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows;
     TAGAN_REQUIRE(blocks <= 0x7fffffff && joins <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
     if (A.splits == 1) {
         if (one) k_attn_fwd<T, D, 1, false><<<(unsigned)blocks, 64, 0, s>>>(A);
