@@ -119,18 +119,25 @@ struct Tile {
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
 
+    // The thread's chunk, made anew at each use: kept over a loop, the addresses of all steps would cost registers that
+    // the accumulators need.
+    __device__ static __forceinline__ int here() {
+        int t = threadIdx.x & 63;
+        asm volatile("" : "+v"(t));
+        return t;
+    }
     // rows [0, rows) of a tile from global rows `stride` bytes apart, `valid` of them and `bytes` of each there
     template <int ROWS, int WAVES>
     __device__ static __forceinline__ void fill(char* lds, const T* base, uint32_t stride, int valid, uint32_t bytes) {
         const uint32_t records = valid > 0 ? (uint32_t)(valid - 1) * stride + bytes : 0u;
         const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)records, 0x00027000);
-        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = here();
         constexpr int STEPS = ROWS * CPR / (64 * WAVES);
         static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int first = (s * WAVES + wave) * 64;
-            const int ci = first + (threadIdx.x & 63);
+            const int ci = first + lane;
             const int r = ci / CPR;
             const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
             const uint32_t at = off < bytes ? (uint32_t)r * stride + off : 0x7ffffff0u;   // past the bound: zeros
@@ -145,13 +152,13 @@ struct Tile {
         const int lt = (int)(((uint32_t)(rem + valid - 1) * magic) >> 20);
         const uint32_t span = valid > 0 ? (uint32_t)lt * tok + (uint32_t)(G - 1) * head + bytes : 0u;
         const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)span, 0x00027000);
-        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = here();
         constexpr int STEPS = ROWS * CPR / (64 * WAVES);
         static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             const int first = (s * WAVES + wave) * 64;
-            const int ci = first + (threadIdx.x & 63);
+            const int ci = first + lane;
             const int r = ci / CPR;
             const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
             const uint32_t x = (uint32_t)(rem + r), t = (x * magic) >> 20, g = x - t * (uint32_t)G;
@@ -160,36 +167,50 @@ struct Tile {
         }
     }
 
-    // operand of rows `row0 + l % 32`, features 16 c + 8 (l / 32) .. + 7
-    __device__ static __forceinline__ void rows(Frag<T>& f, const char* lds, int row0, int c) {
-        const int l = threadIdx.x & 63, r = row0 + (l & 31), h = l >> 5;
+    // Where a lane reads, for row (or run) 0 of a tile.  swz is linear in the bits of the row and chunks are whole powers
+    // of two, so every other address is one exclusive or with a constant and a constant offset; made anew for each tile,
+    // these cost less than the registers that all addresses would take over the loop.
+    struct At {
+        int row, col;
+    };
+    __device__ static __forceinline__ At at() {
+        const int l = here(), h = l >> 5;
+        At p;
         if constexpr (sizeof(T) == 2) {
-            const uint4 u = *(const uint4*)(lds + r * ROW + (((2 * c + h) ^ swz(r)) << 4));
+            // transposed: a lane addresses 4 features of one row; within 16 lanes the 4 x 16 block comes back transposed
+            const int s = l & 15, r = 4 * h + (s >> 2);
+            p.row = (l & 31) * ROW + ((h ^ swz(l & 31)) << 4);
+            p.col = r * ROW + (((((l & 16) >> 3) + ((s & 3) >> 1)) ^ swz(r)) << 4) + (s & 1) * 8;
+        } else {
+            p.row = (l & 31) * ROW + (((2 * h) ^ swz(l & 31)) << 4);
+            p.col = 4 * h * ROW + ((((l & 31) >> 2) ^ swz(4 * h)) << 4) + (l & 3) * 4;
+        }
+        return p;
+    }
+    // operand of rows row0 + l % 32, features 16 c + 8 (l / 32) .. + 7
+    __device__ static __forceinline__ void rows(Frag<T>& f, const char* lds, At p, int row0, int c) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 u = *(const uint4*)(lds + (p.row ^ (c << 5)) + row0 * ROW);
             f.u[0] = u.x; f.u[1] = u.y; f.u[2] = u.z; f.u[3] = u.w;
         } else {
-            const float4 a = *(const float4*)(lds + r * ROW + (((4 * c + 2 * h) ^ swz(r)) << 4));
-            const float4 b = *(const float4*)(lds + r * ROW + (((4 * c + 2 * h + 1) ^ swz(r)) << 4));
+            const float4 a = *(const float4*)(lds + (p.row ^ (c << 6)) + row0 * ROW);
+            const float4 b = *(const float4*)(lds + (p.row ^ (c << 6) ^ 16) + row0 * ROW);
             f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w;
             f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
         }
     }
     // transposed operand: features 32 db + l % 32, rows row0 + 4 h + j % 4 + 8 (j / 4)
-    __device__ static __forceinline__ void cols(Frag<T>& f, char* lds, int row0, int db) {
-        const int l = threadIdx.x & 63, h = l >> 5;
+    __device__ static __forceinline__ void cols(Frag<T>& f, char* lds, At p, int row0, int db) {
         if constexpr (sizeof(T) == 2) {
-            // a lane addresses 4 features of one row; within 16 lanes the 4 x 16 block comes back transposed
-            const int s = l & 15, c = 32 * db + (l & 16) + 4 * (s & 3);
-            const int r = row0 + 4 * h + (s >> 2), r2 = r + 8;
-            char* a = lds + r * ROW + (((c >> 3) ^ swz(r)) << 4) + (c & 7) * 2;
-            char* b = lds + r2 * ROW + (((c >> 3) ^ swz(r2)) << 4) + (c & 7) * 2;
+            char* a = lds + (p.col ^ (db << 6)) + row0 * ROW;
+            char* b = lds + (p.col ^ (db << 6) ^ (swz(8) << 4)) + (row0 + 8) * ROW;
             f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TAGAN_LDS(s16x4, a));
             f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(TAGAN_LDS(s16x4, b));
         } else {
-            const int c = 32 * db + (l & 31);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int r = row0 + 4 * h + (j & 3) + 8 * (j >> 2);
-                f.v[j] = *(const float*)(lds + r * ROW + (((c >> 2) ^ swz(r)) << 4) + (c & 3) * 4);
+                const int r = (j & 3) + 8 * (j >> 2);
+                f.v[j] = *(const float*)(lds + (p.col ^ (db << 7) ^ (swz(r) << 4)) + (row0 + r) * ROW);
             }
         }
     }
@@ -249,7 +270,8 @@ struct Strides {
 struct AttnArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dq, *dk, *dv;
-    float *lse, *delta;
+    float* lse;
+    float2* stat;       // backward: (log-sum-exp, rowsum(dO O)) of each row
     Strides qs, ks, vs, os, dos, dqs, dks, dvs;
     const int32_t *offs_q, *offs_k;   // packed: [n_seq + 1]; null: a cache
     const int32_t* lens;              // cache: [batch] keys of each
@@ -400,14 +422,15 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     float m = -INFINITY, base = 0.f, l = 0.f;   // largest score of the base, that in powers of two, sum over it
 
     int wild_from = 0x7fffffff;                // first key of the tiles that were tamed
-    const auto load = [&](char* kb, char* vb, int kt) {
+    const auto load = [&](char* kb, char* vb, int kt) __attribute__((always_inline)) {
         const int valid = min(KT, kend - kt);
         TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
         TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
     };
-    const auto tile = [&](char* ks, char* vs, int kt) {
+    const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
         if (min(kt + KT, kend) > block_least && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
         if (kt >= wave_last) return;
+        const typename TL::At at = TL::at();
         f32x16 s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -416,7 +439,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 Frag<T> kf;
-                TL::rows(kf, ks, 32 * b, c);
+                TL::rows(kf, ks, at, 32 * b, c);
                 mma(s[b], kf, qf[c]);
             }
         }
@@ -468,7 +491,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> vf;
-                    TL::cols(vf, vs, 32 * b + 16 * x, d);
+                    TL::cols(vf, vs, at, 32 * b + 16 * x, d);
                     mma(o[d], vf, pf);
                 }
             }
@@ -579,13 +602,14 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ
-// Rows as in the forward; also writes delta = rowsum(dO O) for the key kernel that follows on the stream.
+// Rows as in the forward; also writes (log-sum-exp, delta = rowsum(dO O)) of each row for the key kernel that follows on
+// the stream.
 template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dq(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
-    __shared__ __align__(16) char ks[KT * TL::ROW];
-    __shared__ __align__(16) char vs[KT * TL::ROW];
+    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[KT * TL::ROW];
+    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[KT * TL::ROW];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int hk = (int)(blockIdx.x % A.kv_heads);
     const int64_t tiles = gridDim.x / A.kv_heads;
@@ -632,7 +656,7 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
     float lse = INFINITY;
     if (mine) {
         lse = A.lse[tok * A.heads + head];
-        if (half == 0) A.delta[tok * A.heads + head] = delta;
+        if (half == 0) A.stat[tok * A.heads + head] = make_float2(lse, delta);
     }
     f32x16 dq[ND];
 #pragma unroll
@@ -640,13 +664,14 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
 
-    for (int kt = 0; kt < kend; kt += KT) {
-        __syncthreads();
+    const auto load = [&](char* kb, char* vb, int kt) __attribute__((always_inline)) {
         const int valid = min(KT, kend - kt);
-        TL::template fill<KT, WAVES>(ks, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
-        TL::template fill<KT, WAVES>(vs, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
-        tiles_ready();
-        if (kt >= wave_last) continue;
+        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+    };
+    const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
+        if (kt >= wave_last) return;
+        const typename TL::At at = TL::at();
         const bool masked = kt + KT > wave_least;
         const int lim = see - kt - 4 * half;
 #pragma unroll
@@ -657,9 +682,9 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 Frag<T> kf, vf;
-                TL::rows(kf, ks, 32 * b, c);
+                TL::rows(kf, ks, at, 32 * b, c);
                 mma(s, kf, qf[c]);
-                TL::rows(vf, vs, 32 * b, c);
+                TL::rows(vf, vs, at, 32 * b, c);
                 mma(dp, vf, gf[c]);
             }
 #pragma unroll
@@ -679,11 +704,21 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> kf;
-                    TL::cols(kf, ks, 32 * b + 16 * x, d);
+                    TL::cols(kf, ks, at, 32 * b + 16 * x, d);
                     mma(dq[d], kf, pf);
                 }
             }
         }
+    };
+    if (kend > 0) load(ks0, vs0, 0);
+    for (int kt = 0; kt < kend; kt += 2 * KT) {
+        tiles_ready();
+        if (kt + KT < kend) load(ks1, vs1, kt + KT);
+        tile(ks0, vs0, kt);
+        if (kt + KT >= kend) break;
+        tiles_ready();
+        if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
+        tile(ks1, vs1, kt + KT);
     }
     if (!mine) return;
     T* DQ = (T*)A.dq + tok * A.dqs.tok + head * A.dqs.head;
@@ -699,16 +734,21 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dq(AttnArgs A) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
-// A wave has 32 keys (in its lanes) and passes over the rows that see them, QT at a time for the whole block.
-template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) k_attn_dkv(AttnArgs A) {
+// A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
+// those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
+// the block is what bounds the longest block: the first keys of a long causal sequence are seen by every row of the group.
+template <typename T, int D, int WK, int WR>
+__global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dkv(AttnArgs A) {
     typedef Tile<T, D> TL;
-    // rows of a tile: 32, or 64 where 32 would leave lanes of the direct loads without a chunk
-    constexpr int QT = TL::ROW >= 128 ? 32 : 64, NC = D / 16, ND = D / 32, KEYS = 32 * WAVES;
-    __shared__ __align__(16) char qs[QT * TL::ROW];
-    __shared__ __align__(16) char gs[QT * TL::ROW];
-    __shared__ __align__(16) float st[2][QT];          // log-sum-exp and delta of the rows
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    // rows of a tile: 32 to a row wave, and enough for a chunk to every lane of the direct loads
+    constexpr int WAVES = WK * WR, NC = D / 16, ND = D / 32, KEYS = 32 * WK;
+    constexpr int LEAST = 1024 * WAVES / TL::ROW, QT = 32 * WR > LEAST ? 32 * WR : LEAST;
+    constexpr int TILE = QT * TL::ROW;
+    // the keys' own v: in LDS where the accumulators and k leave no registers for it
+    constexpr bool VL = D == 128;
+    __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[TILE], gs1[TILE], st0[QT * 8], st1[QT * 8];
+    __shared__ __align__(16) char vl[VL ? KEYS * TL::ROW : 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
     const int hk = (int)(blockIdx.x % A.kv_heads);
     const int64_t vt = blockIdx.x / A.kv_heads;        // first keys first: with a causal mask most rows see them
     const int i = find_seq(A.offs_k, A.n_seq, A.nk, 1, KEYS, vt);
@@ -724,21 +764,24 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dkv(AttnArgs A) {
         lq = (int)max((int64_t)0, edge(A.offs_q, A.n_seq, A.nq, i + 1) - q0);
     }
     const int G = A.G, past = lk - lq;
-    const int key0 = (int)tile * KEYS, key = key0 + wave * 32 + (lane & 31);
+    const int key0 = (int)tile * KEYS, key = key0 + wk * 32 + (lane & 31);
     const bool mine = key < lk;
     const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
     const T* K = (const T*)A.k + (k0 + key) * A.ks.tok + (int64_t)hk * A.ks.head;
     const T* V = (const T*)A.v + (k0 + key) * A.vs.tok + (int64_t)hk * A.vs.head;
-    Frag<T> kf[NC], vf[NC];
+    Frag<T> kf[NC], vf[VL ? 1 : NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         kf[c].zero();
-        vf[c].zero();
+        if constexpr (!VL) vf[c].zero();
         if (mine && 16 * c + 8 * half < A.dim) {
             load_frag(kf[c], K + 16 * c + 8 * half);
-            load_frag(vf[c], V + 16 * c + 8 * half);
+            if constexpr (!VL) load_frag(vf[c], V + 16 * c + 8 * half);
         }
     }
+    if constexpr (VL)
+        TL::template fill<KEYS, WAVES>(vl, (const T*)A.v + (k0 + key0) * A.vs.tok + (int64_t)hk * A.vs.head,
+                                       (uint32_t)(A.vs.tok * sizeof(T)), min(KEYS, lk - key0), bytes);
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -746,73 +789,120 @@ __global__ void __launch_bounds__(WAVES * 64) k_attn_dkv(AttnArgs A) {
         for (int x = 0; x < 16; ++x) dk[d][x] = dv[d][x] = 0.f;
 
     const int64_t nrows = (int64_t)lq * G;
-    // the first row that sees the block's first key
-    const int64_t rbeg = A.causal ? (int64_t)max(0, key0 - past) * G : 0;
-    for (int64_t r0 = rbeg; r0 < nrows; r0 += QT) {
+    const auto load = [&](char* qs, char* gs, char* st, int64_t r0) __attribute__((always_inline)) {
         const int t0 = (int)(r0 / G), rem = (int)(r0 - (int64_t)t0 * G);
         const int valid = (int)min((int64_t)QT, nrows - r0);
         const int64_t tok = q0 + t0;
-        __syncthreads();
         TL::template fill_rows<QT, WAVES>(qs, (const T*)A.q + tok * A.qs.tok + (int64_t)hk * G * A.qs.head,
                                           (uint32_t)(A.qs.tok * sizeof(T)), (uint32_t)(A.qs.head * sizeof(T)), rem, G,
                                           A.magic, valid, bytes);
         TL::template fill_rows<QT, WAVES>(gs, (const T*)A.dout + tok * A.dos.tok + (int64_t)hk * G * A.dos.head,
                                           (uint32_t)(A.dos.tok * sizeof(T)), (uint32_t)(A.dos.head * sizeof(T)), rem, G,
                                           A.magic, valid, bytes);
-        if ((int)threadIdx.x < QT) {
-            const int r = threadIdx.x;
+        static_assert(QT / 32 <= WAVES, "a wave loads the statistics of 32 rows");
+        // (log-sum-exp, delta) of 32 rows to a load, zeros behind the last row: its q and dO are zeros, so the weight 1
+        // that zeros give adds nothing
+        if (wave < QT / 32) {
+            const int last = (int)(((uint32_t)(rem + valid - 1) * A.magic) >> 20);
+            const float2* base = A.stat + tok * A.heads + (int64_t)hk * G;
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (last * A.heads + G) * 8, 0x00027000);
+            const int r = wave * 32 + (lane >> 1);
             const uint32_t x = (uint32_t)(rem + r), t = (x * A.magic) >> 20, g = x - t * (uint32_t)G;
-            const int64_t at = (tok + t) * A.heads + (int64_t)hk * G + g;
-            st[0][r] = r < valid ? A.lse[at] : INFINITY;
-            st[1][r] = r < valid ? A.delta[at] : 0.f;
+            const uint32_t at = r < valid ? (t * (uint32_t)A.heads + g) * 8 + (lane & 1) * 4 : 0x7ffffff0u;
+            const int to = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(wave) * 256;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, st + to), 4, (int)at, 0, 0, 0);
         }
-        tiles_ready();
-        // rows from `first` on (in local tokens) see this lane's key
-        const bool masked = A.causal && key0 + wave * 32 + 31 > t0 + past;
+    };
+    const auto part = [&](char* qs, char* gs, const char* st, int64_t r0, int q) __attribute__((always_inline)) {
+        const typename TL::At at = TL::at();
+        const int t0 = (int)(r0 / G), rem = (int)(r0 - (int64_t)t0 * G);
+        const bool masked = A.causal && key0 + wk * 32 + 31 > t0 + past;
+        // rows of this lane below it do not see its key
+        const int lim = masked ? (key - past - t0) * G - rem - q - 4 * half : -1;
+        f32x16 s, dp;
 #pragma unroll
-        for (int q = 0; q < QT; q += 32) {
-            f32x16 s, dp;
+        for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+        for (int c = 0; c < NC; ++c) {
+            Frag<T> f;
+            TL::rows(f, qs, at, q, c);
+            mma(s, f, kf[c]);
+            TL::rows(f, gs, at, q, c);
+            if constexpr (VL) TL::rows(vf[0], vl, at, wk * 32, c);
+            mma(dp, f, vf[VL ? 0 : c]);
+        }
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+        for (int x = 0; x < 16; x += 4) {
+            const float4* sp = (const float4*)(st + (q + 2 * x + 4 * half) * 8);
+            const float4 a = sp[0], b = sp[1];
+            const float lx[4] = {a.x, a.z, b.x, b.z}, dx[4] = {a.y, a.w, b.y, b.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[x + y], A.c, -lx[y]));
+                s[x + y] = p;
+                dp[x + y] = p * (dp[x + y] - dx[y]);
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (8 * (x >> 2) + (x & 3) < lim) s[x] = dp[x] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            Frag<T> pf, sf;
+            from_acc(pf, s, 8 * x);
+            from_acc(sf, dp, 8 * x);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
                 Frag<T> f;
-                TL::rows(f, qs, q, c);
-                mma(s, f, kf[c]);
-                TL::rows(f, gs, q, c);
-                mma(dp, f, vf[c]);
+                TL::cols(f, gs, at, q + 16 * x, d);
+                mma(dv[d], f, pf);
+                TL::cols(f, qs, at, q + 16 * x, d);
+                mma(dk[d], f, sf);
             }
-            const int lim = masked ? (key - past - t0) * G - rem - q - 4 * half : -1;   // rows of this lane below it do not see
+        }
+    };
+    const auto rows = [&](char* qs, char* gs, const char* st, int64_t r0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-                const float4 ls = *(const float4*)&st[0][q + 2 * x + 4 * half];
-                const float4 de = *(const float4*)&st[1][q + 2 * x + 4 * half];
-                const float lx[4] = {ls.x, ls.y, ls.z, ls.w}, dx[4] = {de.x, de.y, de.z, de.w};
+        for (int q = 0; q < QT; q += 32 * WR) part(qs, gs, st, r0, q + 32 * wr);
+    };
+    // the first row that sees the block's first key
+    const int64_t rbeg = A.causal ? (int64_t)max(0, key0 - past) * G : 0;
+    if (rbeg < nrows) load(qs0, gs0, st0, rbeg);
+    for (int64_t r0 = rbeg; r0 < nrows; r0 += 2 * QT) {
+        tiles_ready();
+        if (r0 + QT < nrows) load(qs1, gs1, st1, r0 + QT);
+        rows(qs0, gs0, st0, r0);
+        if (r0 + QT >= nrows) break;
+        tiles_ready();
+        if (r0 + 2 * QT < nrows) load(qs0, gs0, st0, r0 + 2 * QT);
+        rows(qs1, gs1, st1, r0 + QT);
+    }
+    if constexpr (WR > 1) {
+        // 64 lanes x 16 ND floats of a wave fit one of the four tiles: one tensor after the other
+        static_assert(WR == 2 && WK == 4 && TILE >= 64 * 16 * ND * 4, "a tile holds a wave's sums");
+        float* const at = (float*)(wk == 0 ? qs0 : wk == 1 ? gs0 : wk == 2 ? qs1 : gs1) + lane;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const bool ok = mine && 2 * x + y >= lim;
-                    const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[x + y], A.c, -lx[y])) : 0.f;
-                    s[x + y] = p;
-                    dp[x + y] = ok ? p * (dp[x + y] - dx[y]) : 0.f;
-                }
+        for (int which = 0; which < 2; ++which) {
+            f32x16* acc = which == 0 ? dv : dk;
+            __syncthreads();
+            if (wr == 1) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) at[(16 * d + x) * 64] = acc[d][x];
             }
+            __syncthreads();
+            if (wr == 0) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                Frag<T> pf, sf;
-                from_acc(pf, s, 8 * x);
-                from_acc(sf, dp, 8 * x);
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    Frag<T> f;
-                    TL::cols(f, gs, q + 16 * x, d);
-                    mma(dv[d], f, pf);
-                    TL::cols(f, qs, q + 16 * x, d);
-                    mma(dk[d], f, sf);
-                }
+                    for (int x = 0; x < 16; ++x) acc[d][x] += at[(16 * d + x) * 64];
             }
         }
     }
-    if (!mine) return;
+    if (!mine || wr > 0) return;
     T* DK = (T*)A.dk + (k0 + key) * A.dks.tok + (int64_t)hk * A.dks.head;
     T* DV = (T*)A.dv + (k0 + key) * A.dvs.tok + (int64_t)hk * A.dvs.head;
 #pragma unroll
@@ -887,8 +977,10 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
     }
     if (A.nk > 0) {
-        if (kone) k_attn_dkv<T, D, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
-        else k_attn_dkv<T, D, 4><<<(unsigned)kblocks, 256, 0, s>>>(A);
+        // fp32 at 128 features: one wave's registers fill a SIMD and v and two tiles 128 KB of LDS
+        constexpr int WR = sizeof(T) == 4 && D == 128 ? 1 : 2;
+        if (kone) k_attn_dkv<T, D, 1, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
+        else k_attn_dkv<T, D, 4, WR><<<(unsigned)kblocks, 256 * WR, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
     }
     return TAGAN_OK;
@@ -971,7 +1063,7 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
 }
 
 size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads) {
-    return nq > 0 && heads > 0 ? (size_t)nq * (size_t)heads * 4 : 0;
+    return nq > 0 && heads > 0 ? (size_t)nq * (size_t)heads * 8 : 0;
 }
 
 int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
@@ -993,7 +1085,7 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     AttnArgs A = {};
     A.q = q; A.k = k; A.v = v; A.o = out; A.dout = dout;
     A.dq = dq; A.dk = dk; A.dv = dv;
-    A.lse = (float*)lse; A.delta = (float*)workspace;
+    A.lse = (float*)lse; A.stat = (float2*)workspace;
     A.qs = {0, q_tok, q_head};
     A.ks = {0, k_tok, k_head};
     A.vs = {0, v_tok, v_head};
