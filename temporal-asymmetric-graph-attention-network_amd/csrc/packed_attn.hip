@@ -353,19 +353,21 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int64_t vt, Seq& s) {
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int D, int WAVES>
 struct Shape {
-    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB); 32 where fp32 doubles that, and for the widest heads of
-    // one-wave blocks, of which five then share a CU's LDS with two tiles each
-    static constexpr int KT = D == 128 && (sizeof(T) == 4 || WAVES == 1) ? 32 : 64;
+    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB), 32 where fp32 doubles that and for one-wave blocks
+    static constexpr int KT = WAVES == 1 || (D == 128 && sizeof(T) == 4) ? 32 : 64;
 };
 
 // A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
-template <typename T, int D, int WAVES, bool SPLIT>
+// STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
+// many more blocks of a CU hide each other's waits.
+template <typename T, int D, int WAVES, bool SPLIT, int STAGES>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_fwd(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     // two buffers, each an object of its own: reads of one do not wait for the loads of the other
-    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[KT * TL::ROW];
-    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[KT * TL::ROW];
+    constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
+    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
+    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     int64_t bid = blockIdx.x;
     int split = 0;
@@ -496,8 +498,16 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
                 }
             }
     };
-    if (kbeg < kend) load(ks0, vs0, kbeg);
-    for (int kt = kbeg; kt < kend; kt += 2 * KT) {
+    if constexpr (STAGES == 1) {
+        for (int kt = kbeg; kt < kend; kt += KT) {
+            __syncthreads();                            // every wave is done with the tile before
+            load(ks0, vs0, kt);
+            tiles_ready();
+            tile(ks0, vs0, kt);
+        }
+    }
+    if (STAGES == 2 && kbeg < kend) load(ks0, vs0, kbeg);
+    for (int kt = kbeg; STAGES == 2 && kt < kend; kt += 2 * KT) {
         tiles_ready();                                  // and every wave is done with the other buffer
         if (kt + KT < kend) load(ks1, vs1, kt + KT);
         tile(ks0, vs0, kt);
@@ -604,12 +614,13 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
 // ------------------------------------------------------------------------------------------------ backward: dQ
 // Rows as in the forward; also writes (log-sum-exp, delta = rowsum(dO O)) of each row for the key kernel that follows on
 // the stream.
-template <typename T, int D, int WAVES>
+template <typename T, int D, int WAVES, int STAGES>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dq(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
-    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[KT * TL::ROW];
-    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[KT * TL::ROW];
+    constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
+    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
+    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int hk = (int)(blockIdx.x % A.kv_heads);
     const int64_t tiles = gridDim.x / A.kv_heads;
@@ -710,8 +721,16 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
             }
         }
     };
-    if (kend > 0) load(ks0, vs0, 0);
-    for (int kt = 0; kt < kend; kt += 2 * KT) {
+    if constexpr (STAGES == 1) {
+        for (int kt = 0; kt < kend; kt += KT) {
+            __syncthreads();
+            load(ks0, vs0, kt);
+            tiles_ready();
+            tile(ks0, vs0, kt);
+        }
+    }
+    if (STAGES == 2 && kend > 0) load(ks0, vs0, 0);
+    for (int kt = 0; STAGES == 2 && kt < kend; kt += 2 * KT) {
         tiles_ready();
         if (kt + KT < kend) load(ks1, vs1, kt + KT);
         tile(ks0, vs0, kt);
@@ -737,7 +756,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
 // A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
 // those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
 // the block is what bounds the longest block: the first keys of a long causal sequence are seen by every row of the group.
-template <typename T, int D, int WK, int WR>
+template <typename T, int D, int WK, int WR, int STAGES>
 __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dkv(AttnArgs A) {
     typedef Tile<T, D> TL;
     // rows of a tile: 32 to a row wave, and enough for a chunk to every lane of the direct loads
@@ -746,7 +765,8 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
     constexpr int TILE = QT * TL::ROW;
     // the keys' own v: in LDS where the accumulators and k leave no registers for it
     constexpr bool VL = D == 128;
-    __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[TILE], gs1[TILE], st0[QT * 8], st1[QT * 8];
+    constexpr int SECOND = STAGES == 2 ? TILE : 16;
+    __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
     __shared__ __align__(16) char vl[VL ? KEYS * TL::ROW : 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
     const int hk = (int)(blockIdx.x % A.kv_heads);
@@ -869,8 +889,16 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
     };
     // the first row that sees the block's first key
     const int64_t rbeg = A.causal ? (int64_t)max(0, key0 - past) * G : 0;
-    if (rbeg < nrows) load(qs0, gs0, st0, rbeg);
-    for (int64_t r0 = rbeg; r0 < nrows; r0 += 2 * QT) {
+    if constexpr (STAGES == 1) {
+        for (int64_t r0 = rbeg; r0 < nrows; r0 += QT) {
+            __syncthreads();
+            load(qs0, gs0, st0, r0);
+            tiles_ready();
+            rows(qs0, gs0, st0, r0);
+        }
+    }
+    if (STAGES == 2 && rbeg < nrows) load(qs0, gs0, st0, rbeg);
+    for (int64_t r0 = rbeg; STAGES == 2 && r0 < nrows; r0 += 2 * QT) {
         tiles_ready();
         if (r0 + QT < nrows) load(qs1, gs1, st1, r0 + QT);
         rows(qs0, gs0, st0, r0);
@@ -881,7 +909,7 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
     }
     if constexpr (WR > 1) {
         // 64 lanes x 16 ND floats of a wave fit one of the four tiles: one tensor after the other
-        static_assert(WR == 2 && WK == 4 && TILE >= 64 * 16 * ND * 4, "a tile holds a wave's sums");
+        static_assert(WR == 2 && WK == 4 && STAGES == 2 && TILE >= 64 * 16 * ND * 4, "a tile holds a wave's sums");
         float* const at = (float*)(wk == 0 ? qs0 : wk == 1 ? gs0 : wk == 2 ? qs1 : gs1) + lane;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -958,8 +986,8 @@ int run_fwd(const AttnArgs& A, hipStream_t s) {
     const int rows = one ? 32 : 128;
     const int64_t blocks = (A.nq * A.G / rows + A.n_seq + 2) * A.kv_heads;
     TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
-    if (one) k_attn_fwd<T, D, 1, false><<<(unsigned)blocks, 64, 0, s>>>(A);
-    else k_attn_fwd<T, D, 4, false><<<(unsigned)blocks, 256, 0, s>>>(A);
+    if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("packed_attn_fwd");
     return TAGAN_OK;
 }
@@ -972,15 +1000,17 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
     TAGAN_REQUIRE(blocks <= 0x7fffffff && kblocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED,
                   "packed_attn_bwd: too many tiles");
     if (A.nq > 0) {
-        if (one) k_attn_dq<T, D, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
-        else k_attn_dq<T, D, 4><<<(unsigned)blocks, 256, 0, s>>>(A);
+        if (one) k_attn_dq<T, D, 1, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+        else k_attn_dq<T, D, 4, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
     }
     if (A.nk > 0) {
-        // fp32 at 128 features: one wave's registers fill a SIMD and v and two tiles 128 KB of LDS
-        constexpr int WR = sizeof(T) == 4 && D == 128 ? 1 : 2;
-        if (kone) k_attn_dkv<T, D, 1, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
-        else k_attn_dkv<T, D, 4, WR><<<(unsigned)kblocks, 256 * WR, 0, s>>>(A);
+        // Two row waves where blocks are few and the longest of them decides; with 4 blocks to a CU and more, smaller ones
+        // keep the CUs busier.  (fp32 at 128 features: one wave's registers fill a SIMD.)
+        constexpr bool TWO = sizeof(T) == 2 || D < 128;
+        if (kone) k_attn_dkv<T, D, 1, 1, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
+        else if (TWO && kblocks < 4 * 256) k_attn_dkv<T, D, 4, TWO ? 2 : 1, 2><<<(unsigned)kblocks, 512, 0, s>>>(A);
+        else k_attn_dkv<T, D, 4, 1, 2><<<(unsigned)kblocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
     }
     return TAGAN_OK;
@@ -1005,13 +1035,13 @@ int run_cached(const AttnArgs& A, hipStream_t s) {
     const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows;
     TAGAN_REQUIRE(blocks <= 0x7fffffff && joins <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
     if (A.splits == 1) {
-        if (one) k_attn_fwd<T, D, 1, false><<<(unsigned)blocks, 64, 0, s>>>(A);
-        else k_attn_fwd<T, D, 4, false><<<(unsigned)blocks, 256, 0, s>>>(A);
+        if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+        else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("cached_attn");
         return TAGAN_OK;
     }
-    if (one) k_attn_fwd<T, D, 1, true><<<(unsigned)blocks, 64, 0, s>>>(A);
-    else k_attn_fwd<T, D, 4, true><<<(unsigned)blocks, 256, 0, s>>>(A);
+    if (one) k_attn_fwd<T, D, 1, true, 2><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, true, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("cached_attn");
     k_attn_join<T, D><<<(unsigned)joins, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("cached_attn (join)");
