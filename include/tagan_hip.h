@@ -631,7 +631,7 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key), so every query i < Lq - Lk sees none;
  * a row without a visible key, or outside every sequence, gives zeros.
  * head_dim: multiples of 8 up to 128; heads / kv_heads <= 512; scale > 0.  Pointers and strides (elements) on 16
- * bytes, feature stride 1, token strides of head_dim to 2^22.
+ * bytes, feature stride 1, token strides of head_dim to 2^21, tokens times heads / kv_heads below 2^31.
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
  * no key is seen.  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero

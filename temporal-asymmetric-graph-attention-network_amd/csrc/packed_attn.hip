@@ -119,51 +119,58 @@ struct Tile {
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
 
-    // The thread's chunk, made anew at each use: kept over a loop, the addresses of all steps would cost registers that
-    // the accumulators need.
-    __device__ static __forceinline__ int here() {
-        int t = threadIdx.x & 63;
-        asm volatile("" : "+v"(t));
-        return t;
+    static constexpr int RPW = 64 / CPR;               // rows of a wave's load
+    static constexpr uint32_t PAST = 0x7ffffff0u;      // an offset behind every bound: the load writes zeros
+
+    // A thread's place in the loads of a tile whose rows are `stride` bytes apart: the row's offset, the chunk's, and
+    // their sum where it lies inside head_dim.
+    struct Lay {
+        uint32_t row, chunk, sum;
+    };
+    template <int WAVES>
+    __device__ static __forceinline__ Lay lay(uint32_t stride, uint32_t bytes) {
+        const int r = (WAVES == 1 ? 0 : (int)threadIdx.x >> 6) * RPW + (threadIdx.x & 63) / CPR;
+        Lay y;
+        y.row = (uint32_t)r * stride;
+        y.chunk = (uint32_t)(((threadIdx.x & 63) % CPR) ^ swz(r)) * 16u;
+        y.sum = y.chunk < bytes ? y.row + y.chunk : PAST;
+        return y;
     }
-    // rows [0, rows) of a tile from global rows `stride` bytes apart, `valid` of them and `bytes` of each there
+    // Rows [0, ROWS) of a tile from global rows `stride` bytes apart, `valid` of them and `bytes` of each there.  Steps lie
+    // whole swizzle periods apart where a step has 16 rows and more, and share a thread's offset.
     template <int ROWS, int WAVES>
-    __device__ static __forceinline__ void fill(char* lds, const T* base, uint32_t stride, int valid, uint32_t bytes) {
-        const uint32_t records = valid > 0 ? (uint32_t)(valid - 1) * stride + bytes : 0u;
-        const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)records, 0x00027000);
-        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = here();
-        constexpr int STEPS = ROWS * CPR / (64 * WAVES);
-        static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
+    __device__ static __forceinline__ void fill(char* lds, const T* base, uint32_t stride, int valid, uint32_t bytes,
+                                                const Lay& y) {
+        constexpr int SR = RPW * WAVES, STEPS = ROWS / SR;
+        static_assert(STEPS * SR == ROWS, "a tile is filled by whole wave loads");
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const int first = (s * WAVES + wave) * 64;
-            const int ci = first + lane;
-            const int r = ci / CPR;
-            const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
-            const uint32_t at = off < bytes ? (uint32_t)r * stride + off : 0x7ffffff0u;   // past the bound: zeros
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + first * 16), 16, (int)at, 0, 0, 0);
+            const uint32_t skip = (uint32_t)(s * SR) * stride;
+            const int records = valid > s * SR ? (int)((uint32_t)(valid - 1 - s * SR) * stride + bytes) : 0;
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc((char*)base + skip, 0, records, 0x00027000);
+            uint32_t at = y.sum;
+            if constexpr (SR % 16 != 0) {
+                const uint32_t c = y.chunk ^ (uint32_t)(swz(s * SR) << 4);
+                at = c < bytes ? y.row + c : PAST;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + (s * WAVES + wave) * 1024), 16, (int)at, 0,
+                                                     0, 0);
         }
     }
-    // the same of packed rows r0 + i = token * G + g; `tok` and `head` strides in bytes
-    template <int ROWS, int WAVES>
-    __device__ static __forceinline__ void fill_rows(char* lds, const T* base, uint32_t tok, uint32_t head, int rem,
-                                                     int G, uint32_t magic, int valid, uint32_t bytes) {
-        // the last valid row bounds the span whatever the order of the strides
-        const int lt = (int)(((uint32_t)(rem + valid - 1) * magic) >> 20);
-        const uint32_t span = valid > 0 ? (uint32_t)lt * tok + (uint32_t)(G - 1) * head + bytes : 0u;
+    // The same of packed rows (token, head of the group), at offsets that `spot` gives for each row of the tile.
+    template <int ROWS, int WAVES, class Spot>
+    __device__ static __forceinline__ void fill_rows(char* lds, const T* base, uint32_t span, uint32_t bytes, Spot spot) {
+        constexpr int SR = RPW * WAVES, STEPS = ROWS / SR;
+        static_assert(STEPS * SR == ROWS, "a tile is filled by whole wave loads");
         const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)span, 0x00027000);
-        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = here();
-        constexpr int STEPS = ROWS * CPR / (64 * WAVES);
-        static_assert(STEPS * 64 * WAVES == ROWS * CPR, "a tile is filled by whole wave loads");
+        const int wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const int first = (s * WAVES + wave) * 64;
-            const int ci = first + lane;
-            const int r = ci / CPR;
-            const uint32_t off = (uint32_t)((ci % CPR) ^ swz(r)) * 16u;
-            const uint32_t x = (uint32_t)(rem + r), t = (x * magic) >> 20, g = x - t * (uint32_t)G;
-            const uint32_t at = (r < valid && off < bytes) ? t * tok + g * head + off : 0x7ffffff0u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + first * 16), 16, (int)at, 0, 0, 0);
+            const int r = s * SR + (WAVES == 1 ? 0 : (int)threadIdx.x >> 6) * RPW + (threadIdx.x & 63) / CPR;
+            const uint32_t c = (uint32_t)(((threadIdx.x & 63) % CPR) ^ swz(r)) * 16u, at = spot(s, r);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, lds + (s * WAVES + wave) * 1024), 16,
+                                                     (int)(at != PAST && c < bytes ? at + c : PAST), 0, 0, 0);
         }
     }
 
@@ -174,7 +181,9 @@ struct Tile {
         int row, col;
     };
     __device__ static __forceinline__ At at() {
-        const int l = here(), h = l >> 5;
+        int l = threadIdx.x & 63;
+        asm volatile("" : "+v"(l));                      // not kept over the loop
+        const int h = l >> 5;
         At p;
         if constexpr (sizeof(T) == 2) {
             // transposed: a lane addresses 4 features of one row; within 16 lanes the 4 x 16 block comes back transposed
@@ -267,6 +276,22 @@ struct Strides {
     int64_t b, tok, head;   // elements
 };
 
+// n / d by a multiplication for n < 2^31: m = ceil(2^(31 + l) / d), l = ceil(log2 d), is off by less than 2^l / d <= 2
+// parts of n / 2^(31 + l) < 2^-l <= 1 / d
+struct Div {
+    uint32_t d, m;
+    int l;
+};
+Div div_by(int64_t d) {
+    Div v = {(uint32_t)d, 0u, 0};
+    while ((1ll << v.l) < d) ++v.l;
+    v.m = (uint32_t)(((1ull << (31 + v.l)) + (uint64_t)d - 1) / (uint64_t)d);
+    return v;
+}
+__device__ __forceinline__ int quot(int n, const Div& v) {
+    return (int)(((uint64_t)(uint32_t)n * v.m) >> (31 + v.l));
+}
+
 struct AttnArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dq, *dk, *dv;
@@ -277,7 +302,7 @@ struct AttnArgs {
     const int32_t* lens;              // cache: [batch] keys of each
     int64_t nq, nk;                   // packed: tokens in all; cache: new tokens and capacity of each
     int32_t n_seq, heads, kv_heads, G, dim, causal, splits;
-    uint32_t magic;                   // (x * magic) >> 20 = x / G for x < G + 256 (G <= 512)
+    Div by_g, by_kv, by_splits, by_tiles;   // of the group, the key heads, the splits, a cache's tiles to a sequence
     float c;                          // scale * log2(e)
     float scale;
     float* part;                      // splits: [split][row of batch][D + 4]
@@ -286,21 +311,20 @@ struct AttnArgs {
 // One sequence and where its rows lie.  Rows outside every sequence belong to two more that see no key (the run before
 // the first offset and the run behind the last), so they get zeros.
 struct Seq {
-    int64_t q0, k0;    // first token, first key (elements of the token axis)
-    int32_t lq, lk, index;
-    int32_t tile;      // tile of this sequence
+    int q0, k0;        // first token, first key
+    int lq, lk, index;
+    int tile;          // tile of this sequence
 };
 
-__device__ __forceinline__ int64_t edge(const int32_t* offs, int n_seq, int64_t n, int i) {
+__device__ __forceinline__ int edge(const int32_t* offs, int n_seq, int n, int i) {
     if (i == 0) return 0;
     if (i == n_seq + 2) return n;
-    const int64_t e = offs[i - 1];
-    return e < 0 ? 0 : (e > n ? n : e);
+    return max(0, min(n, offs[i - 1]));
 }
 
 // The sequence of virtual tile vt: sequence i starts at floor(edge_i * mul / tile) + i, which leaves each room for
 // ceil(length * mul / tile) tiles.  64 probes to a step of the search.
-__device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int64_t n, int mul, int tile, int64_t vt) {
+__device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int n, int mul, int tile, int vt) {
     int lo = 0, count = n_seq + 2;
     while (count > 1) {
         const int step = (count + 63) / 64;
@@ -314,40 +338,59 @@ __device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int64_t 
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
-__device__ __forceinline__ int64_t tile_of(const int32_t* offs, int n_seq, int64_t n, int mul, int tile, int64_t vt,
-                                           int i) {
-    return vt - (edge(offs, n_seq, n, i) * mul / tile + i);
-}
-
 // rows of a query tile: sequence, false where the tile is none
 template <int ROWS>
-__device__ __forceinline__ bool locate(const AttnArgs& A, int64_t vt, Seq& s) {
+__device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
     if (A.offs_q == nullptr) {
-        const int64_t tiles = (A.nq * A.G + ROWS - 1) / ROWS;
-        s.index = (int)(vt / tiles);
-        s.tile = (int)(vt - s.index * tiles);
+        s.index = quot(vt, A.by_tiles);
+        s.tile = vt - s.index * (int)A.by_tiles.d;
         s.lq = (int)A.nq;
         s.q0 = s.k0 = 0;
-        const int n = A.lens[s.index];
-        s.lk = n < 0 ? 0 : (int)min((int64_t)n, A.nk);
+        s.lk = max(0, min((int)A.nk, A.lens[s.index]));
         return true;
     }
-    const int i = find_seq(A.offs_q, A.n_seq, A.nq, A.G, ROWS, vt);
-    const int64_t t = tile_of(A.offs_q, A.n_seq, A.nq, A.G, ROWS, vt, i);
-    s.q0 = edge(A.offs_q, A.n_seq, A.nq, i);
-    const int64_t lq = edge(A.offs_q, A.n_seq, A.nq, i + 1) - s.q0;
-    if (lq <= 0 || t * ROWS >= lq * A.G) return false;
-    s.lq = (int)lq;
-    s.tile = (int)t;
+    const int nq = (int)A.nq, i = find_seq(A.offs_q, A.n_seq, nq, A.G, ROWS, vt);
+    s.q0 = edge(A.offs_q, A.n_seq, nq, i);
+    s.lq = edge(A.offs_q, A.n_seq, nq, i + 1) - s.q0;
+    s.tile = vt - (s.q0 * A.G / ROWS + i);
+    if (s.lq <= 0 || s.tile * ROWS >= s.lq * A.G) return false;
     s.index = 0;
     s.k0 = 0;
     s.lk = 0;
     if (i >= 1 && i <= A.n_seq) {
-        s.k0 = edge(A.offs_k, A.n_seq, A.nk, i);
-        const int64_t lk = edge(A.offs_k, A.n_seq, A.nk, i + 1) - s.k0;
-        s.lk = lk < 0 ? 0 : (int)lk;
+        s.k0 = edge(A.offs_k, A.n_seq, (int)A.nk, i);
+        s.lk = max(0, edge(A.offs_k, A.n_seq, (int)A.nk, i + 1) - s.k0);
     }
     return true;
+}
+
+// The rows of a wave and what they see.  Counts of rows (tokens times the group) stay below 2^31.
+struct Rows {
+    int nrows, r0, row, token, g, past;
+    bool mine;
+    int see;                           // keys of this lane's row
+    int most, least;                   // keys that some row of the block sees, and that all of its rows see
+    int wave_most, wave_least;         // of the wave's 32 rows; wave_least is 0 where rows are missing
+};
+template <int ROWS>
+__device__ __forceinline__ Rows rows_of(const AttnArgs& A, const Seq& sq) {
+    const int lane = threadIdx.x & 63, wave = ROWS == 32 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    Rows R;
+    R.nrows = sq.lq * A.G;
+    R.r0 = sq.tile * ROWS;
+    R.row = R.r0 + wave * 32 + (lane & 31);
+    R.mine = R.row < R.nrows;
+    R.token = quot(R.row, A.by_g);
+    R.g = R.row - R.token * A.G;
+    R.past = sq.lk - sq.lq;            // keys before the first query's own
+    const auto keys = [&](int row) { return A.causal ? min(sq.lk, max(0, quot(row, A.by_g) + R.past + 1)) : sq.lk; };
+    R.see = !R.mine ? 0 : (A.causal ? min(sq.lk, max(0, R.token + R.past + 1)) : sq.lk);
+    R.most = keys(min(R.r0 + ROWS, R.nrows) - 1);
+    R.least = keys(R.r0);
+    const int w0 = R.r0 + wave * 32;
+    R.wave_least = w0 + 31 >= R.nrows ? 0 : keys(w0);
+    R.wave_most = w0 >= R.nrows ? 0 : keys(min(w0 + 32, R.nrows) - 1);
+    return R;
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -368,53 +411,38 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
     __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
     __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    int64_t bid = blockIdx.x;
-    int split = 0;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    int bid = blockIdx.x, split = 0, tiles = quot(gridDim.x, A.by_kv);
     if constexpr (SPLIT) {
-        split = (int)(bid % A.splits);
-        bid /= A.splits;
+        const int rest = quot(bid, A.by_splits);
+        split = bid - rest * A.splits;
+        bid = rest;
+        tiles = quot(tiles, A.by_splits);
     }
-    const int hk = (int)(bid % A.kv_heads);
-    // last tiles first: with a causal mask they have the most keys
-    const int64_t tiles = (int64_t)gridDim.x / A.kv_heads / (SPLIT ? A.splits : 1);
+    // key heads side by side (with 8 of them each XCD keeps to one), last tiles first: when causal they have the most keys
+    const int vt = quot(bid, A.by_kv), hk = bid - vt * A.kv_heads;
     Seq sq;
-    if (!locate<ROWS>(A, tiles - 1 - bid / A.kv_heads, sq)) return;
-
-    const int G = A.G;
-    const int64_t nrows = (int64_t)sq.lq * G;
-    const int64_t r0 = (int64_t)sq.tile * ROWS;
-    const int64_t row = r0 + wave * 32 + (lane & 31);
-    const bool mine = row < nrows;
-    const int token = (int)(row / G), g = (int)(row - (int64_t)token * G);
-    const int past = sq.lk - sq.lq;       // keys before the first query's own
-    // keys that this lane's row, and that the whole block, can see
-    const int see = !mine ? 0 : (A.causal ? min(sq.lk, max(0, token + past + 1)) : sq.lk);
-    const int last_tok = (int)((min(r0 + ROWS, nrows) - 1) / G);
-    int kend = A.causal ? min(sq.lk, max(0, last_tok + past + 1)) : sq.lk;
-    int kbeg = 0;
+    if (!locate<ROWS>(A, tiles - 1 - vt, sq)) return;
+    const Rows R = rows_of<ROWS>(A, sq);
+    int kbeg = 0, kend = R.most;
     if constexpr (SPLIT) {
-        const int per = ((kend + A.splits - 1) / A.splits + KT - 1) / KT * KT;
-        kbeg = min(kend, split * per);
-        kend = min(kend, kbeg + per);
+        const int per = (quot(kend + A.splits - 1, A.by_splits) + KT - 1) / KT * KT;
+        kbeg = min((int64_t)kend, (int64_t)split * per);
+        kend = min((int64_t)kend, (int64_t)kbeg + per);
     }
-    const int block_least = A.causal ? min(sq.lk, max(0, (int)(r0 / G) + past + 1)) : sq.lk;
-    // the least and the most that a row of this wave sees: whole tiles before the least need no mask
-    const int64_t w0 = r0 + wave * 32;
-    const int first_tok = (int)(w0 / G);
-    const int wave_least = w0 + 31 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, first_tok + past + 1)) : sq.lk);
-    const int wave_last = w0 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, (int)((min(w0 + 32, nrows) - 1) / G) + past + 1)) : sq.lk);
-
-    const T* Q = (const T*)A.q + (int64_t)sq.index * A.qs.b + (sq.q0 + token) * A.qs.tok + (int64_t)(hk * G + g) * A.qs.head;
-    const T* K = (const T*)A.k + (int64_t)sq.index * A.ks.b + sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
-    const T* V = (const T*)A.v + (int64_t)sq.index * A.vs.b + sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
-    const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
+    const T* Q = (const T*)A.q + (int64_t)sq.index * A.qs.b + (int64_t)(sq.q0 + R.token) * A.qs.tok +
+                 (int64_t)(hk * A.G + R.g) * A.qs.head;
+    const T* K = (const T*)A.k + (int64_t)sq.index * A.ks.b + (int64_t)sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + (int64_t)sq.index * A.vs.b + (int64_t)sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
+    const uint32_t bytes = (uint32_t)A.dim * sizeof(T), kstep = (uint32_t)(A.ks.tok * sizeof(T)),
+                   vstep = (uint32_t)(A.vs.tok * sizeof(T));
+    const auto klay = TL::template lay<WAVES>(kstep, bytes), vlay = TL::template lay<WAVES>(vstep, bytes);
 
     Frag<T> qf[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         qf[c].zero();
-        if (mine && 16 * c + 8 * half < A.dim) load_frag(qf[c], Q + 16 * c + 8 * half);
+        if (R.mine && 16 * c + 8 * half < A.dim) load_frag(qf[c], Q + 16 * c + 8 * half);
     }
     f32x16 o[ND];
 #pragma unroll
@@ -424,15 +452,15 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     float m = -INFINITY, base = 0.f, l = 0.f;   // largest score of the base, that in powers of two, sum over it
 
     int wild_from = 0x7fffffff;                // first key of the tiles that were tamed
+    const typename TL::At at = TL::at();
     const auto load = [&](char* kb, char* vb, int kt) __attribute__((always_inline)) {
         const int valid = min(KT, kend - kt);
-        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
-        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, kstep, valid, bytes, klay);
+        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, vstep, valid, bytes, vlay);
     };
     const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
-        if (min(kt + KT, kend) > block_least && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
-        if (kt >= wave_last) return;
-        const typename TL::At at = TL::at();
+        if (min(kt + KT, kend) > R.least && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
+        if (kt >= R.wave_most) return;
         f32x16 s[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -445,9 +473,9 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
                 mma(s[b], kf, qf[c]);
             }
         }
-        const bool masked = kt + KT > wave_least || kt + KT > kend;
+        const bool masked = kt + KT > R.wave_least || kt + KT > kend;
         if (masked) {
-            const int lim = min(see, kend) - kt - 4 * half;   // keys of this lane below it are visible
+            const int lim = min(R.see, kend) - kt - 4 * half;   // keys of this lane below it are visible
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -506,20 +534,22 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
             tile(ks0, vs0, kt);
         }
     }
-    if (STAGES == 2 && kbeg < kend) load(ks0, vs0, kbeg);
-    for (int kt = kbeg; STAGES == 2 && kt < kend; kt += 2 * KT) {
-        tiles_ready();                                  // and every wave is done with the other buffer
-        if (kt + KT < kend) load(ks1, vs1, kt + KT);
-        tile(ks0, vs0, kt);
-        if (kt + KT >= kend) break;
-        tiles_ready();
-        if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
-        tile(ks1, vs1, kt + KT);
+    else {
+        if (kbeg < kend) load(ks0, vs0, kbeg);
+        for (int kt = kbeg; kt < kend; kt += 2 * KT) {
+            tiles_ready();                              // and every wave is done with the other buffer
+            if (kt + KT < kend) load(ks1, vs1, kt + KT);
+            tile(ks0, vs0, kt);
+            if (kt + KT >= kend) break;
+            tiles_ready();
+            if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
+            tile(ks1, vs1, kt + KT);
+        }
     }
 #pragma unroll 1
     for (int key = wild_from; key < kend; ++key) {
         const T* value = V + (int64_t)key * A.vs.tok;
-        const bool seen = key < see;
+        const bool seen = key < R.see;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -530,10 +560,11 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
             }
     }
     l = half_sum(l);
-    if (!mine) return;
+    if (!R.mine) return;
     if constexpr (SPLIT) {
         // unnormalised sums with their maximum (in powers of two) and total
-        float* p = A.part + (((int64_t)split * A.n_seq + sq.index) * A.kv_heads + hk) * nrows * (D + 4) + row * (D + 4);
+        float* p = A.part + (((int64_t)split * A.n_seq + sq.index) * A.kv_heads + hk) * R.nrows * (D + 4) +
+                   (int64_t)R.row * (D + 4);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -542,7 +573,8 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
         if (half == 0) *(float2*)(p + D) = make_float2(base, l);
     } else {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        T* O = (T*)A.out + (int64_t)sq.index * A.os.b + (sq.q0 + token) * A.os.tok + (int64_t)(hk * G + g) * A.os.head;
+        T* O = (T*)A.out + (int64_t)sq.index * A.os.b + (int64_t)(sq.q0 + R.token) * A.os.tok +
+               (int64_t)(hk * A.G + R.g) * A.os.head;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -553,7 +585,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
             }
         // +inf where no key is seen: exp2(s - lse) is 0 in the backward
         if (A.lse && half == 0)
-            A.lse[(sq.q0 + token) * A.heads + hk * G + g] = l == 0.f ? INFINITY : base + __log2f(l);
+            A.lse[(int64_t)(sq.q0 + R.token) * A.heads + hk * A.G + R.g] = l == 0.f ? INFINITY : base + __log2f(l);
     }
 }
 
@@ -621,33 +653,21 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
     __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
     __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const int hk = (int)(blockIdx.x % A.kv_heads);
-    const int64_t tiles = gridDim.x / A.kv_heads;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads;
     Seq sq;
-    if (!locate<ROWS>(A, tiles - 1 - blockIdx.x / A.kv_heads, sq)) return;
-    const int G = A.G;
-    const int64_t nrows = (int64_t)sq.lq * G;
-    const int64_t r0 = (int64_t)sq.tile * ROWS;
-    const int64_t row = r0 + wave * 32 + (lane & 31);
-    const bool mine = row < nrows;
-    const int token = (int)(row / G), g = (int)(row - (int64_t)token * G);
-    const int past = sq.lk - sq.lq;
-    const int see = !mine ? 0 : (A.causal ? min(sq.lk, max(0, token + past + 1)) : sq.lk);
-    const int last_tok = (int)((min(r0 + ROWS, nrows) - 1) / G);
-    const int kend = A.causal ? min(sq.lk, max(0, last_tok + past + 1)) : sq.lk;
-    const int64_t w0 = r0 + wave * 32;
-    const int first_tok = (int)(w0 / G);
-    const int wave_least = w0 + 31 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, first_tok + past + 1)) : sq.lk);
-    const int wave_last = w0 >= nrows ? 0 : (A.causal ? min(sq.lk, max(0, (int)((min(w0 + 32, nrows) - 1) / G) + past + 1)) : sq.lk);
-
-    const int64_t head = hk * G + g, tok = sq.q0 + token;
+    if (!locate<ROWS>(A, quot(gridDim.x, A.by_kv) - 1 - vt, sq)) return;
+    const Rows R = rows_of<ROWS>(A, sq);
+    const int kend = R.most;
+    const int64_t head = hk * A.G + R.g, tok = sq.q0 + R.token;
     const T* Q = (const T*)A.q + tok * A.qs.tok + head * A.qs.head;
     const T* O = (const T*)A.o + tok * A.os.tok + head * A.os.head;
     const T* DO = (const T*)A.dout + tok * A.dos.tok + head * A.dos.head;
-    const T* K = (const T*)A.k + sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
-    const T* V = (const T*)A.v + sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
-    const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
+    const T* K = (const T*)A.k + (int64_t)sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + (int64_t)sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
+    const uint32_t bytes = (uint32_t)A.dim * sizeof(T), kstep = (uint32_t)(A.ks.tok * sizeof(T)),
+                   vstep = (uint32_t)(A.vs.tok * sizeof(T));
+    const auto klay = TL::template lay<WAVES>(kstep, bytes), vlay = TL::template lay<WAVES>(vstep, bytes);
 
     Frag<T> qf[NC], gf[NC];
     float delta = 0.f;
@@ -655,7 +675,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     for (int c = 0; c < NC; ++c) {
         qf[c].zero();
         gf[c].zero();
-        if (mine && 16 * c + 8 * half < A.dim) {
+        if (R.mine && 16 * c + 8 * half < A.dim) {
             Frag<T> of;
             load_frag(qf[c], Q + 16 * c + 8 * half);
             load_frag(gf[c], DO + 16 * c + 8 * half);
@@ -665,7 +685,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     }
     delta = half_sum(delta);
     float lse = INFINITY;
-    if (mine) {
+    if (R.mine) {
         lse = A.lse[tok * A.heads + head];
         if (half == 0) A.stat[tok * A.heads + head] = make_float2(lse, delta);
     }
@@ -675,16 +695,16 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[d][i] = 0.f;
 
+    const typename TL::At at = TL::at();
     const auto load = [&](char* kb, char* vb, int kt) __attribute__((always_inline)) {
         const int valid = min(KT, kend - kt);
-        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, (uint32_t)(A.ks.tok * sizeof(T)), valid, bytes);
-        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, (uint32_t)(A.vs.tok * sizeof(T)), valid, bytes);
+        TL::template fill<KT, WAVES>(kb, K + (int64_t)kt * A.ks.tok, kstep, valid, bytes, klay);
+        TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, vstep, valid, bytes, vlay);
     };
     const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
-        if (kt >= wave_last) return;
-        const typename TL::At at = TL::at();
-        const bool masked = kt + KT > wave_least;
-        const int lim = see - kt - 4 * half;
+        if (kt >= R.wave_most) return;
+        const bool masked = kt + KT > R.wave_least;
+        const int lim = R.see - kt - 4 * half;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             f32x16 s, dp;
@@ -729,17 +749,19 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
             tile(ks0, vs0, kt);
         }
     }
-    if (STAGES == 2 && kend > 0) load(ks0, vs0, 0);
-    for (int kt = 0; STAGES == 2 && kt < kend; kt += 2 * KT) {
-        tiles_ready();
-        if (kt + KT < kend) load(ks1, vs1, kt + KT);
-        tile(ks0, vs0, kt);
-        if (kt + KT >= kend) break;
-        tiles_ready();
-        if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
-        tile(ks1, vs1, kt + KT);
+    else {
+        if (kend > 0) load(ks0, vs0, 0);
+        for (int kt = 0; kt < kend; kt += 2 * KT) {
+            tiles_ready();
+            if (kt + KT < kend) load(ks1, vs1, kt + KT);
+            tile(ks0, vs0, kt);
+            if (kt + KT >= kend) break;
+            tiles_ready();
+            if (kt + 2 * KT < kend) load(ks0, vs0, kt + 2 * KT);
+            tile(ks1, vs1, kt + KT);
+        }
     }
-    if (!mine) return;
+    if (!R.mine) return;
     T* DQ = (T*)A.dq + tok * A.dqs.tok + head * A.dqs.head;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -769,26 +791,22 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
     __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
     __shared__ __align__(16) char vl[VL ? KEYS * TL::ROW : 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
-    const int hk = (int)(blockIdx.x % A.kv_heads);
-    const int64_t vt = blockIdx.x / A.kv_heads;        // first keys first: with a causal mask most rows see them
-    const int i = find_seq(A.offs_k, A.n_seq, A.nk, 1, KEYS, vt);
-    const int64_t tile = tile_of(A.offs_k, A.n_seq, A.nk, 1, KEYS, vt, i);
-    const int64_t k0 = edge(A.offs_k, A.n_seq, A.nk, i);
-    const int64_t lk64 = edge(A.offs_k, A.n_seq, A.nk, i + 1) - k0;
-    if (lk64 <= 0 || tile * KEYS >= lk64) return;
-    const int lk = (int)lk64;
-    int64_t q0 = 0;
-    int lq = 0;
+    // first keys first: with a causal mask most rows see them
+    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads;
+    const int nk = (int)A.nk, i = find_seq(A.offs_k, A.n_seq, nk, 1, KEYS, vt);
+    const int k0 = edge(A.offs_k, A.n_seq, nk, i), lk = edge(A.offs_k, A.n_seq, nk, i + 1) - k0;
+    const int key0 = (vt - (k0 / KEYS + i)) * KEYS;
+    if (lk <= 0 || key0 >= lk) return;
+    int q0 = 0, lq = 0;
     if (i >= 1 && i <= A.n_seq) {
-        q0 = edge(A.offs_q, A.n_seq, A.nq, i);
-        lq = (int)max((int64_t)0, edge(A.offs_q, A.n_seq, A.nq, i + 1) - q0);
+        q0 = edge(A.offs_q, A.n_seq, (int)A.nq, i);
+        lq = max(0, edge(A.offs_q, A.n_seq, (int)A.nq, i + 1) - q0);
     }
-    const int G = A.G, past = lk - lq;
-    const int key0 = (int)tile * KEYS, key = key0 + wk * 32 + (lane & 31);
+    const int G = A.G, past = lk - lq, key = key0 + wk * 32 + (lane & 31);
     const bool mine = key < lk;
     const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
-    const T* K = (const T*)A.k + (k0 + key) * A.ks.tok + (int64_t)hk * A.ks.head;
-    const T* V = (const T*)A.v + (k0 + key) * A.vs.tok + (int64_t)hk * A.vs.head;
+    const T* K = (const T*)A.k + (int64_t)(k0 + key) * A.ks.tok + (int64_t)hk * A.ks.head;
+    const T* V = (const T*)A.v + (int64_t)(k0 + key) * A.vs.tok + (int64_t)hk * A.vs.head;
     Frag<T> kf[NC], vf[VL ? 1 : NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -800,45 +818,74 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
         }
     }
     if constexpr (VL)
-        TL::template fill<KEYS, WAVES>(vl, (const T*)A.v + (k0 + key0) * A.vs.tok + (int64_t)hk * A.vs.head,
-                                       (uint32_t)(A.vs.tok * sizeof(T)), min(KEYS, lk - key0), bytes);
+        TL::template fill<KEYS, WAVES>(vl, (const T*)A.v + (int64_t)(k0 + key0) * A.vs.tok + (int64_t)hk * A.vs.head,
+                                       (uint32_t)(A.vs.tok * sizeof(T)), min(KEYS, lk - key0), bytes,
+                                       TL::template lay<WAVES>((uint32_t)(A.vs.tok * sizeof(T)), bytes));
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int x = 0; x < 16; ++x) dk[d][x] = dv[d][x] = 0.f;
 
-    const int64_t nrows = (int64_t)lq * G;
-    const auto load = [&](char* qs, char* gs, char* st, int64_t r0) __attribute__((always_inline)) {
-        const int t0 = (int)(r0 / G), rem = (int)(r0 - (int64_t)t0 * G);
-        const int valid = (int)min((int64_t)QT, nrows - r0);
-        const int64_t tok = q0 + t0;
-        TL::template fill_rows<QT, WAVES>(qs, (const T*)A.q + tok * A.qs.tok + (int64_t)hk * G * A.qs.head,
-                                          (uint32_t)(A.qs.tok * sizeof(T)), (uint32_t)(A.qs.head * sizeof(T)), rem, G,
-                                          A.magic, valid, bytes);
-        TL::template fill_rows<QT, WAVES>(gs, (const T*)A.dout + tok * A.dos.tok + (int64_t)hk * G * A.dos.head,
-                                          (uint32_t)(A.dos.tok * sizeof(T)), (uint32_t)(A.dos.head * sizeof(T)), rem, G,
-                                          A.magic, valid, bytes);
-        static_assert(QT / 32 <= WAVES, "a wave loads the statistics of 32 rows");
-        // (log-sum-exp, delta) of 32 rows to a load, zeros behind the last row: its q and dO are zeros, so the weight 1
-        // that zeros give adds nothing
+    // Tiles of whole tokens, so that a row's (token, head of the group) is the same in every tile and its offset is kept:
+    // QT / G tokens; groups wider than a tile take as many tiles to a token, the last of them part empty.
+    const bool wide = G > QT;
+    const int tokens = wide ? 1 : QT / G, pieces = wide ? (G + QT - 1) / QT : 1;
+    const uint32_t qtok = (uint32_t)(A.qs.tok * sizeof(T)), qhead = (uint32_t)(A.qs.head * sizeof(T)),
+                   gtok = (uint32_t)(A.dos.tok * sizeof(T)), ghead = (uint32_t)(A.dos.head * sizeof(T));
+    constexpr int SR = TL::RPW * WAVES, STEPS = QT / SR;
+    uint32_t qat[STEPS], gat[STEPS];
+    int rt[STEPS];                                     // token of the row in a tile; many where the row is none
+    const int myrow = (WAVES == 1 ? 0 : (int)threadIdx.x >> 6) * TL::RPW + (threadIdx.x & 63) / TL::CPR;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int r = myrow + s * SR, t = wide ? 0 : quot(r, A.by_g), g = r - t * G;
+        rt[s] = t < tokens ? t : 1 << 30;
+        qat[s] = t < tokens ? (uint32_t)t * qtok + (uint32_t)g * qhead : TL::PAST;
+        gat[s] = t < tokens ? (uint32_t)t * gtok + (uint32_t)g * ghead : TL::PAST;
+    }
+    // (log-sum-exp, delta) of 32 rows to a wave
+    const int srow = wave * 32 + (lane >> 1), stok = wide ? 0 : quot(srow, A.by_g);
+    const uint32_t sat = ((uint32_t)stok * (uint32_t)A.heads + (uint32_t)(srow - stok * G)) * 8 + (lane & 1) * 4;
+    static_assert(QT / 32 <= WAVES, "a wave loads the statistics of 32 rows");
+
+    // tile n: tokens [t0, t0 + tokens), from head g0 of the group on
+    const int tbeg = A.causal ? max(0, key0 - past) : 0;       // the first token that sees the block's first key
+    const int ntiles = tbeg < lq ? (lq - tbeg + tokens - 1) / tokens * pieces : 0;
+    const auto load = [&](char* qs, char* gs, char* st, int n) __attribute__((always_inline)) {
+        const int step = wide ? n / pieces : n, t0 = tbeg + step * tokens, g0 = wide ? (n - step * pieces) * QT : 0;
+        const int there = min(tokens, lq - t0), heads = min(QT, G - g0);       // tokens, and heads of a wide token
+        const int64_t tok = q0 + t0, head = (int64_t)hk * G + g0;
+        const bool part = wide ? heads < QT : there < tokens;
+        const auto have = [&](int s, int r) __attribute__((always_inline)) {
+            return !part || (wide ? r < heads : rt[s] < there);
+        };
+        const uint32_t qspan = (uint32_t)(there - 1) * qtok + (uint32_t)((wide ? heads : G) - 1) * qhead + bytes;
+        const uint32_t gspan = (uint32_t)(there - 1) * gtok + (uint32_t)((wide ? heads : G) - 1) * ghead + bytes;
+        TL::template fill_rows<QT, WAVES>(qs, (const T*)A.q + tok * A.qs.tok + head * A.qs.head, qspan, bytes,
+                                          [&](int s, int r) __attribute__((always_inline)) {
+                                              return have(s, r) ? qat[s] : TL::PAST;
+                                          });
+        TL::template fill_rows<QT, WAVES>(gs, (const T*)A.dout + tok * A.dos.tok + head * A.dos.head, gspan, bytes,
+                                          [&](int s, int r) __attribute__((always_inline)) {
+                                              return have(s, r) ? gat[s] : TL::PAST;
+                                          });
+        // zeros where a row is none: its q and dO are zeros, so the weight 1 that zeros give adds nothing
         if (wave < QT / 32) {
-            const int last = (int)(((uint32_t)(rem + valid - 1) * A.magic) >> 20);
-            const float2* base = A.stat + tok * A.heads + (int64_t)hk * G;
-            const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (last * A.heads + G) * 8, 0x00027000);
-            const int r = wave * 32 + (lane >> 1);
-            const uint32_t x = (uint32_t)(rem + r), t = (x * A.magic) >> 20, g = x - t * (uint32_t)G;
-            const uint32_t at = r < valid ? (t * (uint32_t)A.heads + g) * 8 + (lane & 1) * 4 : 0x7ffffff0u;
+            const float2* base = A.stat + tok * A.heads + head;
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)base, 0, ((there - 1) * A.heads + (wide ? heads : G)) * 8, 0x00027000);
+            const bool is = stok < tokens && (wide ? srow < heads : stok < there);
             const int to = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(wave) * 256;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, st + to), 4, (int)at, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TAGAN_LDS(void, st + to), 4, (int)(is ? sat : TL::PAST), 0, 0, 0);
         }
     };
-    const auto part = [&](char* qs, char* gs, const char* st, int64_t r0, int q) __attribute__((always_inline)) {
+    const auto part = [&](char* qs, char* gs, const char* st, int n, int q) __attribute__((always_inline)) {
         const typename TL::At at = TL::at();
-        const int t0 = (int)(r0 / G), rem = (int)(r0 - (int64_t)t0 * G);
+        const int t0 = tbeg + (wide ? n / pieces : n) * tokens;
         const bool masked = A.causal && key0 + wk * 32 + 31 > t0 + past;
-        // rows of this lane below it do not see its key
-        const int lim = masked ? (key - past - t0) * G - rem - q - 4 * half : -1;
+        // rows of this lane below it do not see its key; a wide token's rows are of one token
+        const int lim = !masked ? -1 : wide ? (key > t0 + past ? QT : -1) : (key - past - t0) * G - q - 4 * half;
         f32x16 s, dp;
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
@@ -883,29 +930,28 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
             }
         }
     };
-    const auto rows = [&](char* qs, char* gs, const char* st, int64_t r0) __attribute__((always_inline)) {
+    const auto rows = [&](char* qs, char* gs, const char* st, int n) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < QT; q += 32 * WR) part(qs, gs, st, r0, q + 32 * wr);
+        for (int q = 0; q < QT; q += 32 * WR) part(qs, gs, st, n, q + 32 * wr);
     };
-    // the first row that sees the block's first key
-    const int64_t rbeg = A.causal ? (int64_t)max(0, key0 - past) * G : 0;
     if constexpr (STAGES == 1) {
-        for (int64_t r0 = rbeg; r0 < nrows; r0 += QT) {
+        for (int n = 0; n < ntiles; ++n) {
             __syncthreads();
-            load(qs0, gs0, st0, r0);
+            load(qs0, gs0, st0, n);
             tiles_ready();
-            rows(qs0, gs0, st0, r0);
+            rows(qs0, gs0, st0, n);
         }
-    }
-    if (STAGES == 2 && rbeg < nrows) load(qs0, gs0, st0, rbeg);
-    for (int64_t r0 = rbeg; STAGES == 2 && r0 < nrows; r0 += 2 * QT) {
-        tiles_ready();
-        if (r0 + QT < nrows) load(qs1, gs1, st1, r0 + QT);
-        rows(qs0, gs0, st0, r0);
-        if (r0 + QT >= nrows) break;
-        tiles_ready();
-        if (r0 + 2 * QT < nrows) load(qs0, gs0, st0, r0 + 2 * QT);
-        rows(qs1, gs1, st1, r0 + QT);
+    } else {
+        if (ntiles > 0) load(qs0, gs0, st0, 0);
+        for (int n = 0; n < ntiles; n += 2) {
+            tiles_ready();
+            if (n + 1 < ntiles) load(qs1, gs1, st1, n + 1);
+            rows(qs0, gs0, st0, n);
+            if (n + 1 >= ntiles) break;
+            tiles_ready();
+            if (n + 2 < ntiles) load(qs0, gs0, st0, n + 2);
+            rows(qs1, gs1, st1, n + 1);
+        }
     }
     if constexpr (WR > 1) {
         // 64 lanes x 16 ND floats of a wave fit one of the four tiles: one tensor after the other
@@ -931,8 +977,8 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
         }
     }
     if (!mine || wr > 0) return;
-    T* DK = (T*)A.dk + (k0 + key) * A.dks.tok + (int64_t)hk * A.dks.head;
-    T* DV = (T*)A.dv + (k0 + key) * A.dvs.tok + (int64_t)hk * A.dvs.head;
+    T* DK = (T*)A.dk + (int64_t)(k0 + key) * A.dks.tok + (int64_t)hk * A.dks.head;
+    T* DV = (T*)A.dv + (int64_t)(k0 + key) * A.dvs.tok + (int64_t)hk * A.dvs.head;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -969,12 +1015,10 @@ int check_tensor(const char* what, const char* name, const void* p, const Stride
     TAGAN_REQUIRE(p, TAGAN_ERR_ARG, "%s: %s is null", what, name);
     TAGAN_REQUIRE(aligned(p, s.b, s.tok, s.head, es), TAGAN_ERR_ARG,
                   "%s: %s has to lie on 16 bytes, its strides too", what, name);
-    TAGAN_REQUIRE(s.tok >= dim && s.tok <= (1 << 22) && s.head >= 0 && s.head <= (1ll << 40) && s.b >= 0, TAGAN_ERR_ARG,
+    TAGAN_REQUIRE(s.tok >= dim && s.tok <= (1 << 21) && s.head >= 0 && s.head <= (1ll << 40) && s.b >= 0, TAGAN_ERR_ARG,
                   "%s: %s has token stride %lld, head stride %lld", what, name, (long long)s.tok, (long long)s.head);
     return TAGAN_OK;
 }
-
-uint32_t magic_of(int G) { return ((1u << 20) + (uint32_t)G - 1) / (uint32_t)G; }
 
 #define TAGAN_BY_DIM(T, dim, F)                                    \
     ((dim) <= 32 ? F<T, 32> : (dim) <= 64 ? F<T, 64> : F<T, 128>)
@@ -1005,11 +1049,12 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
     }
     if (A.nk > 0) {
-        // Two row waves where blocks are few and the longest of them decides; with 4 blocks to a CU and more, smaller ones
-        // keep the CUs busier.  (fp32 at 128 features: one wave's registers fill a SIMD.)
-        constexpr bool TWO = sizeof(T) == 2 || D < 128;
+        // Two row waves where blocks are few and the longest of them decides, and for 256-byte rows, whose accumulators
+        // leave two waves to a SIMD in any case; with 4 blocks to a CU and more, smaller ones keep the CUs busier.
+        // (fp32 at 128 features: one wave's registers fill a SIMD.)
+        constexpr bool TWO = sizeof(T) == 2 || D < 128, WIDE = D * sizeof(T) == 256;
         if (kone) k_attn_dkv<T, D, 1, 1, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
-        else if (TWO && kblocks < 4 * 256) k_attn_dkv<T, D, 4, TWO ? 2 : 1, 2><<<(unsigned)kblocks, 512, 0, s>>>(A);
+        else if (WIDE || (TWO && kblocks < 4 * 256)) k_attn_dkv<T, D, 4, TWO ? 2 : 1, 2><<<(unsigned)kblocks, 512, 0, s>>>(A);
         else k_attn_dkv<T, D, 4, 1, 2><<<(unsigned)kblocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
     }
@@ -1066,6 +1111,8 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
                   "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: %lld tokens of %d heads",
+                  (long long)nq, heads);
     if (nq == 0) return TAGAN_OK;
     TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_fwd: null offsets");
     const int es = dtype == TAGAN_F32 ? 4 : 2;
@@ -1085,7 +1132,8 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.nq = nq; A.nk = nk; A.n_seq = n_seq;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
     A.causal = causal != 0; A.splits = 1;
-    A.magic = magic_of(A.G);
+    A.by_g = div_by(A.G);
+    A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     hipStream_t s = as_stream(stream);
     return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_fwd)(A, s)
@@ -1107,6 +1155,8 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
                   "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: %lld tokens of %d heads",
+                  (long long)nq, heads);
     if (nq == 0 && nk == 0) return TAGAN_OK;
     TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_bwd: null offsets");
     TAGAN_REQUIRE(workspace_bytes >= tagan_packed_attn_bwd_workspace(nq, heads) && (nq == 0 || (workspace && lse)),
@@ -1133,7 +1183,8 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.nq = nq; A.nk = nk; A.n_seq = n_seq;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
     A.causal = causal != 0; A.splits = 1;
-    A.magic = magic_of(A.G);
+    A.by_g = div_by(A.G);
+    A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     // a tile of packed rows spans (32 / G + 2) tokens and G heads in 31 bits
     TAGAN_REQUIRE((q_head > do_head ? q_head : do_head) * A.G * es < (1ll << 30), TAGAN_ERR_UNSUPPORTED,
@@ -1162,6 +1213,8 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
                   TAGAN_ERR_ARG, "cached_attn: batch %lld new_len %d capacity %lld", (long long)batch, new_len,
                   (long long)capacity);
     if (batch == 0 || new_len == 0) return TAGAN_OK;
+    TAGAN_REQUIRE((int64_t)new_len * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
+                  "cached_attn: %d new tokens of %d heads", new_len, heads);
     TAGAN_REQUIRE(lens, TAGAN_ERR_ARG, "cached_attn: null lens");
     const int es = dtype == TAGAN_F32 ? 4 : 2;
     AttnArgs A = {};
@@ -1180,10 +1233,13 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
     A.nq = new_len; A.nk = capacity; A.n_seq = (int32_t)batch;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
     A.causal = 1;
-    A.magic = magic_of(A.G);
+    A.by_g = div_by(A.G);
+    A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     const int64_t rows = (int64_t)new_len * A.G;
     A.splits = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
+    A.by_splits = div_by(A.splits);
+    A.by_tiles = div_by((rows + (cache_one(rows) ? 31 : 127)) / (cache_one(rows) ? 32 : 128));
     A.part = (float*)workspace;
     const size_t need = tagan_cached_attn_workspace(batch, new_len, capacity, heads, kv_heads, head_dim);
     TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), TAGAN_ERR_WORKSPACE,

@@ -27,7 +27,7 @@ from ._lib import check, dtype_code, lib, ptr, require_hip, stream_of
 MAX_HEAD_DIM = 128        # attention: multiples of 8 up to this
 MAX_ROTARY_DIM = 256
 MAX_GROUP = 512           # query heads to a key head
-MAX_TOKEN_STRIDE = 1 << 22
+MAX_TOKEN_STRIDE = 1 << 21
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 
