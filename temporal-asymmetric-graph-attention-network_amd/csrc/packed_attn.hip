@@ -34,6 +34,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LAZY = 8.f;
 
+
 // ------------------------------------------------------------------------------------------------ fragments
 template <typename T>
 struct Frag;
@@ -301,7 +302,7 @@ struct AttnArgs {
     const int32_t *offs_q, *offs_k;   // packed: [n_seq + 1]; null: a cache
     const int32_t* lens;              // cache: [batch] keys of each
     int64_t nq, nk;                   // packed: tokens in all; cache: new tokens and capacity of each
-    int32_t n_seq, heads, kv_heads, G, dim, causal, splits;
+    int32_t n_seq, heads, kv_heads, G, dim, causal, splits, ranked;
     Div by_g, by_kv, by_splits, by_tiles;   // of the group, the key heads, the splits, a cache's tiles to a sequence
     float c;                          // scale * log2(e)
     float scale;
@@ -338,6 +339,56 @@ __device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int n, i
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// Heaviest tiles first.  With up to 62 sequences (and the two runs outside them) a lane keeps one of them, and every
+// block finds its own tile: the rank-th in falling order of work, by bisection on the work W.  `first` and `count` give
+// the tiles of the lane's sequence whose work is at least W, which are [first, first + count) in either order of work.
+// A long sequence whose tiles begin last costs the launch a fifth of its time (six histories of 1188 to 4096 tokens, dK
+// and dV: 782 us against 640); the 20 wave sums are a few per cent of a long block, so only launches of few blocks do it,
+// and the row kernels, whose blocks are shorter, lost 8 % by it.
+constexpr int ORDERED = 62;
+__device__ __forceinline__ int wave_sum_int(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max_int(int x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+// most: no tile has more work
+template <class AtLeast>
+__device__ __forceinline__ bool ranked(int rank, int most, AtLeast at_least, int& seq, int& tile) {
+    int first, lo = 0, hi = most + 1;          // count(lo) > rank >= count(hi)
+    if (wave_sum_int(at_least(0, first)) <= rank) return false;
+    int above = 0;
+    while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2, n = wave_sum_int(at_least(mid, first));
+        if (n > rank) lo = mid;
+        else {
+            hi = mid;
+            above = n;
+        }
+    }
+    // the tiles of work lo exactly: in order of the sequences, those of one in order of their numbers
+    int f_hi;
+    const int n_hi = at_least(hi, f_hi), n = at_least(lo, first) - n_hi;
+    int before = n;                            // inclusive sum over the lanes
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(before, o, 64);
+        if (lane >= o) before += up;
+    }
+    const int left = rank - above;
+    seq = __ffsll((long long)__ballot(before > left)) - 1;
+    const int own = first < f_hi || n_hi == 0 ? first : f_hi + n_hi;   // where the exact ones begin
+    tile = __shfl(own, seq, 64) + left - __shfl(before - n, seq, 64);
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    return true;
+}
+
 // rows of a query tile: sequence, false where the tile is none
 template <int ROWS>
 __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
@@ -350,9 +401,9 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
         return true;
     }
     const int nq = (int)A.nq, i = find_seq(A.offs_q, A.n_seq, nq, A.G, ROWS, vt);
+    s.tile = vt - (edge(A.offs_q, A.n_seq, nq, i) * A.G / ROWS + i);
     s.q0 = edge(A.offs_q, A.n_seq, nq, i);
     s.lq = edge(A.offs_q, A.n_seq, nq, i + 1) - s.q0;
-    s.tile = vt - (s.q0 * A.G / ROWS + i);
     if (s.lq <= 0 || s.tile * ROWS >= s.lq * A.G) return false;
     s.index = 0;
     s.k0 = 0;
@@ -396,15 +447,16 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs& A, const Seq& sq) {
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int D, int WAVES>
 struct Shape {
-    // keys of a tile: 64 (K and V of 128 bf16 features: 32 KB), 32 where fp32 doubles that and for one-wave blocks
-    static constexpr int KT = WAVES == 1 || (D == 128 && sizeof(T) == 4) ? 32 : 64;
+    // keys of a tile: 64; 32 for one-wave blocks and for 128 features, whose scores then leave the forward three waves to
+    // a SIMD (ragged prompts 345 -> 315 us)
+    static constexpr int KT = WAVES == 1 || D == 128 ? 32 : 64;
 };
 
 // A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
 // STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
 // many more blocks of a CU hide each other's waits.
 template <typename T, int D, int WAVES, bool SPLIT, int STAGES>
-__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_fwd(AttnArgs A) {
+__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3) k_attn_fwd(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     // two buffers, each an object of its own: reads of one do not wait for the loads of the other
@@ -463,16 +515,17 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
         if (kt >= R.wave_most) return;
         f32x16 s[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
                 Frag<T> kf;
                 TL::rows(kf, ks, at, 32 * b, c);
                 mma(s[b], kf, qf[c]);
             }
-        }
         const bool masked = kt + KT > R.wave_least || kt + KT > kend;
         if (masked) {
             const int lim = min(R.see, kend) - kt - 4 * half;   // keys of this lane below it are visible
@@ -648,7 +701,7 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
 // the stream.
 template <typename T, int D, int WAVES, int STAGES>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dq(AttnArgs A) {
-    constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    constexpr int KT = WAVES == 1 || (D == 128 && sizeof(T) == 4) ? 32 : 64, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
     __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
@@ -791,11 +844,30 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
     __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
     __shared__ __align__(16) char vl[VL ? KEYS * TL::ROW : 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
-    // first keys first: with a causal mask most rows see them
-    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads;
-    const int nk = (int)A.nk, i = find_seq(A.offs_k, A.n_seq, nk, 1, KEYS, vt);
-    const int k0 = edge(A.offs_k, A.n_seq, nk, i), lk = edge(A.offs_k, A.n_seq, nk, i + 1) - k0;
-    const int key0 = (vt - (k0 / KEYS + i)) * KEYS;
+    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads, nk = (int)A.nk;
+    int i, tile;
+    if (A.ranked) {
+        int slq = 0, slk = 0;
+        if (lane < A.n_seq + 2) {
+            slk = max(0, edge(A.offs_k, A.n_seq, nk, lane + 1) - edge(A.offs_k, A.n_seq, nk, lane));
+            if (lane >= 1 && lane <= A.n_seq)
+                slq = max(0, edge(A.offs_q, A.n_seq, (int)A.nq, lane + 1) - edge(A.offs_q, A.n_seq, (int)A.nq, lane));
+        }
+        const int tiles = (slk + KEYS - 1) / KEYS, most = wave_max_int(slq);
+        // tile t is seen by lq - max(0, t KEYS - past) tokens (all of them when not causal), 0 at least
+        const bool found = ranked(vt, most, [&](int w, int& first) {
+            first = 0;
+            if (w <= 0) return tiles;
+            if (slq < w) return 0;
+            const int span = slk - w;          // lq - w + past
+            return !A.causal ? tiles : span < 0 ? 0 : min(tiles, span / KEYS + 1);
+        }, i, tile);
+        if (!found) return;
+    } else {
+        i = find_seq(A.offs_k, A.n_seq, nk, 1, KEYS, vt);
+        tile = vt - (edge(A.offs_k, A.n_seq, nk, i) / KEYS + i);
+    }
+    const int k0 = edge(A.offs_k, A.n_seq, nk, i), lk = edge(A.offs_k, A.n_seq, nk, i + 1) - k0, key0 = tile * KEYS;
     if (lk <= 0 || key0 >= lk) return;
     int q0 = 0, lq = 0;
     if (i >= 1 && i <= A.n_seq) {
@@ -954,25 +1026,39 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
         }
     }
     if constexpr (WR > 1) {
-        // 64 lanes x 16 ND floats of a wave fit one of the four tiles: one tensor after the other
-        static_assert(WR == 2 && WK == 4 && STAGES == 2 && TILE >= 64 * 16 * ND * 4, "a tile holds a wave's sums");
-        float* const at = (float*)(wk == 0 ? qs0 : wk == 1 ? gs0 : wk == 2 ? qs1 : gs1) + lane;
+        // 64 lanes x 16 ND floats of a wave to a slot of the tiles: one tensor after the other
+        constexpr int SLOT = 64 * 16 * ND * 4, PER = TILE / SLOT;
+        static_assert(STAGES == 2 && 4 * PER >= (WR - 1) * WK, "the tiles hold the waves' sums");
+        const auto slot = [&](int w) __attribute__((always_inline)) {
+            const int n = (w - 1) * WK + wk, t = n / PER;
+            return (float*)((t == 0 ? qs0 : t == 1 ? gs0 : t == 2 ? qs1 : gs1) + n % PER * SLOT) + 4 * lane;
+        };
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             f32x16* acc = which == 0 ? dv : dk;
             __syncthreads();
-            if (wr == 1) {
+            if (wr > 0) {
+                float* at = slot(wr);
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) at[(16 * d + x) * 64] = acc[d][x];
+                    for (int x = 0; x < 16; x += 4)
+                        *(float4*)(at + (16 * d + x) * 64) =
+                            make_float4(acc[d][x], acc[d][x + 1], acc[d][x + 2], acc[d][x + 3]);
             }
             __syncthreads();
             if (wr == 0) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+                for (int w = 1; w < WR; ++w) {
+                    const float* at = slot(w);
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) acc[d][x] += at[(16 * d + x) * 64];
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int x = 0; x < 16; x += 4) {
+                            const float4 v = *(const float4*)(at + (16 * d + x) * 64);
+                            acc[d][x] += v.x; acc[d][x + 1] += v.y; acc[d][x + 2] += v.z; acc[d][x + 3] += v.w;
+                        }
+                }
             }
         }
     }
@@ -1036,29 +1122,35 @@ int run_fwd(const AttnArgs& A, hipStream_t s) {
     return TAGAN_OK;
 }
 
+template <typename T, int D, int WK, int WR, int STAGES>
+int launch_dkv(AttnArgs A, hipStream_t s) {
+    const int64_t blocks = (A.nk / (32 * WK) + A.n_seq + 2) * A.kv_heads;
+    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
+    A.ranked = A.n_seq >= 2 && A.n_seq <= ORDERED && blocks < 16 * 256;
+    k_attn_dkv<T, D, WK, WR, STAGES><<<(unsigned)blocks, 64 * WK * WR, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
+    return TAGAN_OK;
+}
+
 template <typename T, int D>
 int run_bwd(const AttnArgs& A, hipStream_t s) {
     const bool one = A.nq * A.G < (int64_t)64 * A.n_seq, kone = A.nk < (int64_t)64 * A.n_seq;
     const int64_t blocks = (A.nq * A.G / (one ? 32 : 128) + A.n_seq + 2) * A.kv_heads;
-    const int64_t kblocks = (A.nk / (kone ? 32 : 128) + A.n_seq + 2) * A.kv_heads;
-    TAGAN_REQUIRE(blocks <= 0x7fffffff && kblocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED,
-                  "packed_attn_bwd: too many tiles");
+    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
     if (A.nq > 0) {
         if (one) k_attn_dq<T, D, 1, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
         else k_attn_dq<T, D, 4, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
     }
-    if (A.nk > 0) {
-        // Two row waves where blocks are few and the longest of them decides, and for 256-byte rows, whose accumulators
-        // leave two waves to a SIMD in any case; with 4 blocks to a CU and more, smaller ones keep the CUs busier.
-        // (fp32 at 128 features: one wave's registers fill a SIMD.)
-        constexpr bool TWO = sizeof(T) == 2 || D < 128, WIDE = D * sizeof(T) == 256;
-        if (kone) k_attn_dkv<T, D, 1, 1, 1><<<(unsigned)kblocks, 64, 0, s>>>(A);
-        else if (WIDE || (TWO && kblocks < 4 * 256)) k_attn_dkv<T, D, 4, TWO ? 2 : 1, 2><<<(unsigned)kblocks, 512, 0, s>>>(A);
-        else k_attn_dkv<T, D, 4, 1, 2><<<(unsigned)kblocks, 256, 0, s>>>(A);
-        TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
-    }
-    return TAGAN_OK;
+    if (A.nk == 0) return TAGAN_OK;
+    const int64_t wide = (A.nk / 128 + A.n_seq + 2) * A.kv_heads;
+    // Two row waves where blocks are few and the longest of them decides, and for 256-byte rows, whose accumulators leave
+    // two waves to a SIMD in any case; with 4 blocks to a CU and more, smaller ones keep the CUs busier (48 histories to
+    // 512 tokens, 64 features: 84 us against 111).  fp32 at 128 features: one wave's registers fill a SIMD.
+    if (kone) return launch_dkv<T, D, 1, 1, 1>(A, s);
+    if constexpr (sizeof(T) == 4 && D == 128) return launch_dkv<T, D, 4, 1, 2>(A, s);
+    else if (wide >= 4 * 256 && D * sizeof(T) < 256) return launch_dkv<T, D, 4, 1, 2>(A, s);
+    else return launch_dkv<T, D, 4, 2, 2>(A, s);
 }
 
 // Splits of the key axis for a cache: enough one-wave blocks for 8 to a CU, and at least 128 keys of the capacity to
@@ -1109,8 +1201,8 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           float* lse, void* stream) {
     int rc = check_shape("packed_attn_fwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
-                  "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
+                  TAGAN_ERR_ARG, "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
     TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0) return TAGAN_OK;
@@ -1153,8 +1245,8 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("packed_attn_bwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff && nk <= 0x7fffffff, TAGAN_ERR_ARG,
-                  "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
+                  TAGAN_ERR_ARG, "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
     TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0 && nk == 0) return TAGAN_OK;

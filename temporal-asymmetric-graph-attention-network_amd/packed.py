@@ -302,7 +302,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
           "q %s, k %s and v %s", tuple(q.shape), tuple(k.shape), tuple(v.shape))
     _heads(q.shape[1], k.shape[1])
     scale = _dims(q.shape[2], scale)
-    _need(max(q.shape[0], k.shape[0]) < 1 << 31, "%d and %d tokens", q.shape[0], k.shape[0])
+    _need(max(q.shape[0] * (q.shape[1] // k.shape[1]), k.shape[0]) < (1 << 31) - 1024, "%d and %d tokens", q.shape[0],
+          k.shape[0])
     offsets = _index(offsets, "offsets")
     _need(offsets.shape[0] >= 1, "offsets are empty")
     if offsets_k is None:

@@ -151,12 +151,13 @@ def test_packed_fwd_entry(kw, status):
     assert _fwd(_lib.lib(), **kw) == status
 
 
-def _bwd(L, ws=A, size=4 * 4 * 4, lse=A, head=16, heads=4):
+def _bwd(L, ws=A, size=None, lse=A, head=16, heads=4):
+    size = L.tagan_packed_attn_bwd_workspace(4, heads) if size is None else size
     return L.tagan_packed_attn_bwd(0, 1, 4, 4, heads, 2, 16, A, 64, head, A, 32, 16, A, 32, 16, A, A, 1, 0.25, A, 64,
                                    16, lse, A, 64, 16, A, 64, 16, A, 32, 16, A, 32, 16, ws, size, None)
 
 
-@pytest.mark.parametrize("kw, status", [(dict(size=63), -4), (dict(ws=None), -4), (dict(lse=None), -4),
+@pytest.mark.parametrize("kw, status", [(dict(size=4 * 4 * 8 - 1), -4), (dict(ws=None), -4), (dict(lse=None), -4),
                                         (dict(head=1 << 28), -2), (dict(heads=3), -1)])
 def test_packed_bwd_entry(kw, status):
     assert _bwd(_lib.lib(), **kw) == status
