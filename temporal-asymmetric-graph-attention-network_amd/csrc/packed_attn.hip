@@ -1096,9 +1096,14 @@ int check_shape(const char* what, int dtype, int64_t heads, int64_t kv_heads, in
     return TAGAN_OK;
 }
 
-// strides that a tile's 32-bit offsets and 16-byte loads can take; tiled: read through buffer descriptors
-int check_tensor(const char* what, const char* name, const void* p, const Strides& s, int32_t dim, int es) {
+// Strides that a tile's 32-bit offsets and 16-byte loads can take.  An axis of one step is never stepped over: its stride
+// is anything.
+int check_tensor(const char* what, const char* name, const void* p, Strides& s, int64_t nb, int64_t nt, int64_t nh,
+                 int32_t dim, int es) {
     TAGAN_REQUIRE(p, TAGAN_ERR_ARG, "%s: %s is null", what, name);
+    if (nb <= 1) s.b = 0;
+    if (nt <= 1) s.tok = dim;
+    if (nh <= 1) s.head = dim;
     TAGAN_REQUIRE(aligned(p, s.b, s.tok, s.head, es), TAGAN_ERR_ARG,
                   "%s: %s has to lie on 16 bytes, its strides too", what, name);
     TAGAN_REQUIRE(s.tok >= dim && s.tok <= (1 << 21) && s.head >= 0 && s.head <= (1ll << 40) && s.b >= 0, TAGAN_ERR_ARG,
@@ -1153,12 +1158,12 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
     else return launch_dkv<T, D, 4, 2, 2>(A, s);
 }
 
-// Splits of the key axis for a cache: enough one-wave blocks for 8 to a CU, and at least 128 keys of the capacity to
+// Splits of the key axis for a cache: enough one-wave blocks for 16 to a CU, and at least 64 keys of the capacity to
 // each (the lengths themselves are on the device; a split divides the length it finds there)
 int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity, bool one) {
     const int64_t blocks = batch * kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128));
     const int64_t want = ((one ? 4096 : 1024) + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = (capacity + 127) / 128;
+    const int64_t most = (capacity + 63) / 64;
     const int64_t n = want < most ? want : most;
     return (int)(n < 1 ? 1 : n > MAX_SPLITS ? MAX_SPLITS : n);
 }
@@ -1214,12 +1219,12 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.ks = {0, k_tok, k_head};
     A.vs = {0, v_tok, v_head};
     A.os = {0, o_tok, o_head};
-    if ((rc = check_tensor("packed_attn_fwd", "q", q, A.qs, head_dim, es)) != TAGAN_OK) return rc;
+    if ((rc = check_tensor("packed_attn_fwd", "q", q, A.qs, 1, nq, heads, head_dim, es)) != TAGAN_OK) return rc;
     if (nk > 0) {
-        if ((rc = check_tensor("packed_attn_fwd", "k", k, A.ks, head_dim, es)) != TAGAN_OK) return rc;
-        if ((rc = check_tensor("packed_attn_fwd", "v", v, A.vs, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("packed_attn_fwd", "k", k, A.ks, 1, nk, kv_heads, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("packed_attn_fwd", "v", v, A.vs, 1, nk, kv_heads, head_dim, es)) != TAGAN_OK) return rc;
     }
-    if ((rc = check_tensor("packed_attn_fwd", "out", out, A.os, head_dim, es)) != TAGAN_OK) return rc;
+    if ((rc = check_tensor("packed_attn_fwd", "out", out, A.os, 1, nq, heads, head_dim, es)) != TAGAN_OK) return rc;
     A.offs_q = offsets_q; A.offs_k = offsets_k;
     A.nq = nq; A.nk = nk; A.n_seq = n_seq;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
@@ -1266,11 +1271,13 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.dqs = {0, dq_tok, dq_head};
     A.dks = {0, dk_tok, dk_head};
     A.dvs = {0, dv_tok, dv_head};
-    const struct { const char* name; const void* p; const Strides& s; int64_t n; } all[] = {
-        {"q", q, A.qs, nq}, {"out", out, A.os, nq}, {"dout", dout, A.dos, nq}, {"dq", dq, A.dqs, nq},
-        {"k", k, A.ks, nk}, {"v", v, A.vs, nk}, {"dk", dk, A.dks, nk}, {"dv", dv, A.dvs, nk}};
+    const struct { const char* name; const void* p; Strides& s; int64_t n; int32_t h; } all[] = {
+        {"q", q, A.qs, nq, heads}, {"out", out, A.os, nq, heads}, {"dout", dout, A.dos, nq, heads},
+        {"dq", dq, A.dqs, nq, heads}, {"k", k, A.ks, nk, kv_heads}, {"v", v, A.vs, nk, kv_heads},
+        {"dk", dk, A.dks, nk, kv_heads}, {"dv", dv, A.dvs, nk, kv_heads}};
     for (const auto& x : all)
-        if (x.n > 0 && (rc = check_tensor("packed_attn_bwd", x.name, x.p, x.s, head_dim, es)) != TAGAN_OK) return rc;
+        if (x.n > 0 && (rc = check_tensor("packed_attn_bwd", x.name, x.p, x.s, 1, x.n, x.h, head_dim, es)) != TAGAN_OK)
+            return rc;
     A.offs_q = offsets_q; A.offs_k = offsets_k;
     A.nq = nq; A.nk = nk; A.n_seq = n_seq;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
@@ -1279,7 +1286,7 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     // a tile of packed rows spans (32 / G + 2) tokens and G heads in 31 bits
-    TAGAN_REQUIRE((q_head > do_head ? q_head : do_head) * A.G * es < (1ll << 30), TAGAN_ERR_UNSUPPORTED,
+    TAGAN_REQUIRE((A.qs.head > A.dos.head ? A.qs.head : A.dos.head) * A.G * es < (1ll << 30), TAGAN_ERR_UNSUPPORTED,
                   "packed_attn_bwd: head strides %lld and %lld", (long long)q_head, (long long)do_head);
     hipStream_t s = as_stream(stream);
     return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_bwd)(A, s)
@@ -1315,12 +1322,12 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
     A.ks = {k_b, k_tok, k_head};
     A.vs = {v_b, v_tok, v_head};
     A.os = {o_b, o_tok, o_head};
-    if ((rc = check_tensor("cached_attn", "q", q, A.qs, head_dim, es)) != TAGAN_OK) return rc;
+    if ((rc = check_tensor("cached_attn", "q", q, A.qs, batch, new_len, heads, head_dim, es)) != TAGAN_OK) return rc;
     if (capacity > 0) {
-        if ((rc = check_tensor("cached_attn", "k_cache", k_cache, A.ks, head_dim, es)) != TAGAN_OK) return rc;
-        if ((rc = check_tensor("cached_attn", "v_cache", v_cache, A.vs, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("cached_attn", "k_cache", k_cache, A.ks, batch, capacity, kv_heads, head_dim, es)) != TAGAN_OK) return rc;
+        if ((rc = check_tensor("cached_attn", "v_cache", v_cache, A.vs, batch, capacity, kv_heads, head_dim, es)) != TAGAN_OK) return rc;
     }
-    if ((rc = check_tensor("cached_attn", "out", out, A.os, head_dim, es)) != TAGAN_OK) return rc;
+    if ((rc = check_tensor("cached_attn", "out", out, A.os, batch, new_len, heads, head_dim, es)) != TAGAN_OK) return rc;
     A.lens = lens;
     A.nq = new_len; A.nk = capacity; A.n_seq = (int32_t)batch;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;

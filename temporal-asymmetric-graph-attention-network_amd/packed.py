@@ -22,7 +22,7 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import check, dtype_code, lib, ptr, require_hip, stream_of
+from ._lib import check, dtype_code, lib, require_hip
 
 MAX_HEAD_DIM = 128        # attention: multiples of 8 up to this
 MAX_ROTARY_DIM = 256
@@ -32,70 +32,71 @@ _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3
 
 
 # ----------------------------------------------------------------------------- arguments
-def _need(ok: bool, text: str, *args) -> None:
-    if not ok:
-        raise ValueError(text % args)
+# A serving step's time is the host's: the checks below build no message and no list unless something is wrong.
+def _refuse(text: str, *args):
+    raise ValueError(text % args)
+
+
+def _shapes(*tensors) -> str:
+    return ", ".join("None" if t is None else str(tuple(t.shape)) for t in tensors)
 
 
 def _on_device(first: torch.Tensor, *rest) -> None:
     require_hip(first, *rest)
     for t in rest:
         if t is not None and t.device != first.device:
-            raise ValueError("tensors on %s and %s" % (first.device, t.device))
+            _refuse("tensors on %s and %s", first.device, t.device)
 
 
 def _storage(first: torch.Tensor, *rest) -> None:
-    for t in (first,) + rest:
-        if t is not None and t.dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError("float32 or bfloat16 is wanted, got %s" % t.dtype)
-        if t is not None and t.dtype != first.dtype:
-            raise TypeError("tensors of %s and %s" % (first.dtype, t.dtype))
+    dtype = first.dtype
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
+        raise TypeError("float32 or bfloat16 is wanted, got %s" % dtype)
+    for t in rest:
+        if t is not None and t.dtype is not dtype:
+            raise TypeError("tensors of %s and %s" % (dtype, t.dtype))
 
 
 def _index(t: torch.Tensor, name: str, size: Optional[int] = None) -> torch.Tensor:
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         raise TypeError("%s has to be int32, got %s" % (name, t.dtype))
-    _need(t.dim() == 1 and (size is None or t.shape[0] == size), "%s has shape %s", name, tuple(t.shape))
+    if t.dim() != 1 or (size is not None and t.shape[0] != size):
+        _refuse("%s has shape %s", name, _shapes(t))
     return t.contiguous()
 
 
 def _heads(heads: int, kv_heads: int) -> None:
-    _need(kv_heads >= 1 and heads >= kv_heads and heads % kv_heads == 0 and heads // kv_heads <= MAX_GROUP,
-          "%d query heads over %d key heads", heads, kv_heads)
+    if kv_heads < 1 or heads < kv_heads or heads % kv_heads or heads // kv_heads > MAX_GROUP:
+        _refuse("%d query heads over %d key heads", heads, kv_heads)
 
 
-def _strides(t: torch.Tensor):
-    """Element strides of all axes but the last; an axis of one step gets its dense stride."""
-    got, dense = [], t.shape[-1]
-    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        got.append(s if n > 1 else dense)
-        dense *= max(n, 1)
-    return got[::-1]
-
-
-def _fits(t: torch.Tensor, spread: int = 1 << 30) -> bool:
-    """Whether the attention kernels can read t in place: 16-byte runs, whole rows, a tile within 32-bit offsets."""
+def _fits(t: torch.Tensor) -> bool:
+    """Whether the attention kernels can read t in place: 16-byte runs, whole rows, a tile within 32-bit offsets (an axis
+    of one step is never stepped over)."""
     if t.stride(-1) != 1 or t.data_ptr() % 16:
         return False
-    st, es = _strides(t), t.element_size()
-    return (all(s >= 0 and s * es % 16 == 0 for s in st) and t.shape[-1] <= st[-2] <= MAX_TOKEN_STRIDE
-            and st[-1] * t.shape[-2] * es < spread)
+    es, d, heads, tokens = t.element_size(), t.shape[-1], t.shape[-2], t.shape[-3]
+    return (all(n <= 1 or (s >= 0 and s * es % 16 == 0) for n, s in zip(t.shape[:-1], t.stride()))
+            and (tokens <= 1 or d <= t.stride(-3) <= MAX_TOKEN_STRIDE)
+            and (heads <= 1 or t.stride(-2) * heads * es < 1 << 30))
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    if _fits(t):
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and t.shape[-1] * t.shape[-2] <= MAX_TOKEN_STRIDE:
         return t
-    t = t.contiguous()
     return t if _fits(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _run(name: str, t: torch.Tensor, *args) -> None:
     """The C entry on the device and current stream of t."""
-    if t.device.index == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, stream_of(t)), name)
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            check(getattr(lib(), name)(*args, stream_of(t)), name)
+        with torch.cuda.device(index):
+            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 # ----------------------------------------------------------------------------- rotary positions
@@ -110,18 +111,21 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     least ``fast`` turns over ``original_len``, divides those that make at most ``slow``, goes linearly (in turns)
     between, and returns the scale 0.1 ln(factor) + 1.  The scale is 1 otherwise.
     """
-    _need(dim >= 2 and dim % 2 == 0, "%d features cannot be turned in pairs", dim)
-    _need(base > 0 and math.isfinite(base) and factor >= 1 and math.isfinite(factor), "base %g, factor %g", base,
-          factor)
+    if dim < 2 or dim % 2:
+        _refuse("%d features cannot be turned in pairs", dim)
+    if not (base > 0 and math.isfinite(base) and factor >= 1 and math.isfinite(factor)):
+        _refuse("base %g, factor %g", base, factor)
     if scaling == "base":
-        _need(dim > 2, "the base cannot be raised for %d features", dim)
+        if dim == 2:
+            _refuse("the base cannot be raised for 2 features")
         base = base * factor ** (dim / (dim - 2))
     freq = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
     scale = 1.0
     if scaling == "linear":
         freq = freq / factor
     elif scaling == "parts":
-        _need(fast > slow and original_len >= 1, "turns %g to %g over %d positions", slow, fast, original_len)
+        if not (fast > slow and original_len >= 1):
+            _refuse("turns %g to %g over %d positions", slow, fast, original_len)
         turns = original_len * freq / (2 * math.pi)
         keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
         freq = freq * keep + freq / factor * (1 - keep)
@@ -134,23 +138,25 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
 def _frequencies(inv_freq: torch.Tensor, dim: int) -> torch.Tensor:
     if inv_freq.dtype not in (torch.float64, torch.float32):
         raise TypeError("inv_freq has to be float64 or float32, got %s" % inv_freq.dtype)
-    _need(inv_freq.dim() == 1 and 1 <= inv_freq.shape[0] and 2 * inv_freq.shape[0] <= dim <= MAX_ROTARY_DIM,
-          "%s frequencies for heads of %d features (up to %d)", tuple(inv_freq.shape), dim, MAX_ROTARY_DIM)
+    if inv_freq.dim() != 1 or not 2 <= 2 * inv_freq.shape[0] <= dim <= MAX_ROTARY_DIM:
+        _refuse("%s frequencies for heads of %d features (up to %d)", _shapes(inv_freq), dim, MAX_ROTARY_DIM)
     return inv_freq.to(torch.float64).contiguous()
 
 
 def _turn(q, k, positions, inv_freq, interleaved, scale, inverse):
-    n, _, d = q.shape
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
-    if n == 0:
-        return qo, ko
+    n, heads, d = q.shape
     q = q if q.stride(-1) == 1 else q.contiguous()
-    k = k if k is None or k.stride(-1) == 1 else k.contiguous()
-    hk = k.shape[1] if k is not None else 0
-    _run("tagan_rotary", q, dtype_code(q), n, q.shape[1], hk, d, 2 * inv_freq.shape[0], ptr(q), *_strides(q), ptr(k),
-         *(_strides(k) if hk else (0, 0)), ptr(positions), _POS_TYPES[positions.dtype], ptr(inv_freq), scale,
-         interleaved, inverse, ptr(qo), *_strides(qo), ptr(ko), *(_strides(ko) if hk else (0, 0)))
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ko, hk = None, 0
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        ko, hk = torch.empty_like(k, memory_format=torch.contiguous_format), k.shape[1]
+    if n:
+        kin = (k.data_ptr(), *k.stride()[:2]) if hk else (None, 0, 0)
+        kout = (ko.data_ptr(), hk * d, d) if hk else (None, 0, 0)
+        _run("tagan_rotary", q, dtype_code(q), n, heads, hk, d, 2 * inv_freq.shape[0], q.data_ptr(), *q.stride()[:2],
+             *kin, positions.data_ptr(), _POS_TYPES[positions.dtype], inv_freq.data_ptr(), scale, interleaved, inverse,
+             qo.data_ptr(), heads * d, d, *kout)
     return qo, ko
 
 
@@ -184,22 +190,28 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     (2i, 2i + 1) with ``interleaved``, times ``scale``; the features behind them are copied.  Angles are formed in
     fp64.  Gradients flow to q and k."""
     _storage(q, k)
-    _need(q.dim() == 3 and (k is None or (k.dim() == 3 and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2])),
-          "q %s and k %s", tuple(q.shape), None if k is None else tuple(k.shape))
-    _need(q.shape[1] >= 1 and (k is None or k.shape[1] >= 1), "no heads")
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        _refuse("q and k: %s", _shapes(q, k))
+    if q.shape[1] < 1 or (k is not None and k.shape[1] < 1):
+        _refuse("no heads: %s", _shapes(q, k))
     if positions.dtype not in _POS_TYPES:
         raise TypeError("positions of %s" % positions.dtype)
-    _need(positions.shape == (q.shape[0],), "%s positions for %d tokens", tuple(positions.shape), q.shape[0])
-    _need(math.isfinite(scale), "scale %g", scale)
+    if positions.dim() != 1 or positions.shape[0] != q.shape[0]:
+        _refuse("%s positions for %d tokens", _shapes(positions), q.shape[0])
+    if not math.isfinite(scale):
+        _refuse("scale %g", scale)
     inv_freq = _frequencies(inv_freq, q.shape[2])
     _on_device(q, k, positions, inv_freq)
     return RotaryFn.apply(q, k, positions.contiguous(), inv_freq, bool(interleaved), float(scale))
 
 
 def _cache(t: torch.Tensor, name: str) -> None:
-    _need(t.dim() == 4, "%s %s: [batch, capacity, heads, features] is wanted", name, tuple(t.shape))
-    _need(not t.requires_grad, "%s is written and read in place: it cannot require a gradient", name)
-    _need(t.stride(-1) == 1, "%s needs unit feature stride", name)
+    if t.dim() != 4:
+        _refuse("%s %s: [batch, capacity, heads, features] is wanted", name, _shapes(t))
+    if t.requires_grad:
+        _refuse("%s is written and read in place: it cannot require a gradient", name)
+    if t.stride(-1) != 1:
+        _refuse("%s needs unit feature stride", name)
 
 
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -213,26 +225,29 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     _storage(q, k, v, k_cache, v_cache)
     _cache(k_cache, "k_cache")
     _cache(v_cache, "v_cache")
-    _need(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape and q.shape[:2] == k.shape[:2]
-          and q.shape[3] == k.shape[3], "q %s, k %s and v %s", tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    if (q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2]
+            or q.shape[3] != k.shape[3]):
+        _refuse("q, k and v: %s", _shapes(q, k, v))
     B, L, heads, d = q.shape
     hk = k.shape[2]
     _heads(heads, hk)
-    _need(k_cache.shape == v_cache.shape and k_cache.shape[0] == B and k_cache.shape[2:] == k.shape[2:],
-          "caches %s and %s for k %s", tuple(k_cache.shape), tuple(v_cache.shape), tuple(k.shape))
+    if k_cache.shape != v_cache.shape or k_cache.shape[0] != B or k_cache.shape[2:] != k.shape[2:]:
+        _refuse("caches and k: %s", _shapes(k_cache, v_cache, k))
     for c in (k_cache, v_cache):
-        _need(all(s > 0 for n, s in zip(c.shape, c.stride()) if n > 1), "a cache with shared rows cannot be written")
+        if 0 in c.stride() and any(n > 1 and s <= 0 for n, s in zip(c.shape, c.stride())):
+            _refuse("a cache with shared rows cannot be written")
     lens = _index(lens, "lens", B)
-    _need(math.isfinite(scale), "scale %g", scale)
+    if not math.isfinite(scale):
+        _refuse("scale %g", scale)
     inv_freq = _frequencies(inv_freq, d)
     _on_device(q, k, v, k_cache, v_cache, lens, inv_freq)
-    q, k, v = (t.detach() if t.stride(-1) == 1 else t.detach().contiguous() for t in (q, k, v))
-    out = torch.empty((B, L, heads, d), dtype=q.dtype, device=q.device)
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q.detach(), k.detach(), v.detach()))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B and L:
-        _run("tagan_rotary_append", q, dtype_code(q), B, L, heads, hk, d, 2 * inv_freq.shape[0], ptr(q), *_strides(q),
-             ptr(k), *_strides(k), ptr(v), *_strides(v), ptr(lens), ptr(inv_freq), float(scale), int(interleaved),
-             ptr(out), *_strides(out), ptr(k_cache), *_strides(k_cache), ptr(v_cache), *_strides(v_cache),
-             k_cache.shape[1])
+        _run("tagan_rotary_append", q, dtype_code(q), B, L, heads, hk, d, 2 * inv_freq.shape[0], q.data_ptr(),
+             *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], lens.data_ptr(),
+             inv_freq.data_ptr(), scale, 1 if interleaved else 0, out.data_ptr(), L * heads * d, heads * d, d,
+             k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[1])
     return out
 
 
@@ -245,13 +260,14 @@ class PackedAttnFn(torch.autograd.Function):
         q, k, v = _dense(q), _dense(k), _dense(v)
         n, heads, d = q.shape
         nk, hk, _ = k.shape
-        out = torch.empty((n, heads, d), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         needs = any(ctx.needs_input_grad[:3])
         lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if needs else None
         if n:
-            _run("tagan_packed_attn_fwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, ptr(q),
-                 *_strides(q), ptr(k), *_strides(k), ptr(v), *_strides(v), ptr(offsets), ptr(offsets_k), int(causal),
-                 scale, ptr(out), *_strides(out), ptr(lse))
+            _run("tagan_packed_attn_fwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, q.data_ptr(),
+                 *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], offsets.data_ptr(),
+                 offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d,
+                 lse.data_ptr() if needs else None)
         if needs:
             ctx.save_for_backward(q, k, v, out, lse, offsets, offsets_k)
             ctx.cfg = (causal, scale)
@@ -265,21 +281,24 @@ class PackedAttnFn(torch.autograd.Function):
         dout = _dense(dout)
         n, heads, d = q.shape
         nk, hk, _ = k.shape
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         if n or nk:
             size = lib().tagan_packed_attn_bwd_workspace(n, heads)
-            ws = torch.empty(max(int(size), 1), dtype=torch.uint8, device=q.device)
-            _run("tagan_packed_attn_bwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, ptr(q),
-                 *_strides(q), ptr(k), *_strides(k), ptr(v), *_strides(v), ptr(offsets), ptr(offsets_k), int(causal),
-                 scale, ptr(out), *_strides(out)[:2], ptr(lse), ptr(dout), *_strides(dout), ptr(dq), *_strides(dq),
-                 ptr(dk), *_strides(dk), ptr(dv), *_strides(dv), ptr(ws), size)
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=q.device)
+            _run("tagan_packed_attn_bwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, q.data_ptr(),
+                 *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], offsets.data_ptr(),
+                 offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d, lse.data_ptr(), dout.data_ptr(),
+                 *dout.stride()[:2], dq.data_ptr(), heads * d, d, dk.data_ptr(), hk * d, d, dv.data_ptr(), hk * d, d,
+                 ws.data_ptr(), size)
         return dq, dk, dv, None, None, None, None
 
 
 def _dims(d: int, scale: Optional[float]) -> float:
-    _need(8 <= d <= MAX_HEAD_DIM and d % 8 == 0, "heads of %d features (a multiple of 8 up to %d)", d, MAX_HEAD_DIM)
+    if d < 8 or d > MAX_HEAD_DIM or d % 8:
+        _refuse("heads of %d features (a multiple of 8 up to %d)", d, MAX_HEAD_DIM)
     scale = d ** -0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale) and scale > 0, "scale %g has to be positive and finite", scale)
+    if not (math.isfinite(scale) and scale > 0):
+        _refuse("scale %g has to be positive and finite", scale)
     return scale
 
 
@@ -298,16 +317,19 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.
     """
     _storage(q, k, v)
-    _need(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and q.shape[2] == k.shape[2],
-          "q %s, k %s and v %s", tuple(q.shape), tuple(k.shape), tuple(v.shape))
-    _heads(q.shape[1], k.shape[1])
-    scale = _dims(q.shape[2], scale)
-    _need(max(q.shape[0] * (q.shape[1] // k.shape[1]), k.shape[0]) < (1 << 31) - 1024, "%d and %d tokens", q.shape[0],
-          k.shape[0])
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        _refuse("q, k and v: %s", _shapes(q, k, v))
+    n, heads, d = q.shape
+    _heads(heads, k.shape[1])
+    scale = _dims(d, scale)
+    if max(n * (heads // k.shape[1]), k.shape[0]) >= (1 << 31) - 1024:
+        _refuse("%d and %d tokens", n, k.shape[0])
     offsets = _index(offsets, "offsets")
-    _need(offsets.shape[0] >= 1, "offsets are empty")
+    if offsets.shape[0] < 1:
+        _refuse("offsets are empty")
     if offsets_k is None:
-        _need(q.shape[0] == k.shape[0], "%d queries and %d keys need offsets_k", q.shape[0], k.shape[0])
+        if n != k.shape[0]:
+            _refuse("%d queries and %d keys need offsets_k", n, k.shape[0])
         offsets_k = offsets
     else:
         offsets_k = _index(offsets_k, "offsets_k", offsets.shape[0])
@@ -321,27 +343,25 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
     ``lens`` [B] int32 counts the cached rows of each history, the L new ones included: query i sees rows
     j < lens[b] - L + 1 + i, and zeros come back where that is none.  Rows from ``lens[b]`` on are not used, whatever
-    they hold.  The caches are read in place (unit feature stride, other strides on 16 bytes).  No autograd."""
+    they hold.  The caches are read in place: unit feature stride, other strides and the start on 16 bytes, token strides
+    up to 2^21 elements (RuntimeError otherwise).  No autograd."""
     _storage(q, k_cache, v_cache)
     _cache(k_cache, "k_cache")
     _cache(v_cache, "v_cache")
-    _need(q.dim() == 4 and k_cache.shape == v_cache.shape and q.shape[0] == k_cache.shape[0]
-          and q.shape[3] == k_cache.shape[3], "q %s and caches %s, %s", tuple(q.shape), tuple(k_cache.shape),
-          tuple(v_cache.shape))
+    if q.dim() != 4 or k_cache.shape != v_cache.shape or q.shape[0] != k_cache.shape[0] or q.shape[3] != k_cache.shape[3]:
+        _refuse("q and caches: %s", _shapes(q, k_cache, v_cache))
     B, L, heads, d = q.shape
     cap, hk = k_cache.shape[1:3]
     _heads(heads, hk)
     scale = _dims(d, scale)
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _need(c.numel() == 0 or _fits(c, 1 << 62), "%s: strides %s cannot be read in place", name, c.stride())
     lens = _index(lens, "lens", B)
     _on_device(q, k_cache, v_cache, lens)
     q = _dense(q.detach())
-    out = torch.empty((B, L, heads, d), dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if B and L:
-        size = int(lib().tagan_cached_attn_workspace(B, L, cap, heads, hk, d))
+        size = lib().tagan_cached_attn_workspace(B, L, cap, heads, hk, d)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-        _run("tagan_cached_attn", q, dtype_code(q), B, L, cap, heads, hk, d, ptr(q), *_strides(q), ptr(k_cache),
-             *_strides(k_cache), ptr(v_cache), *_strides(v_cache), ptr(lens), scale, ptr(out), *_strides(out), ptr(ws),
-             size)
+        _run("tagan_cached_attn", q, dtype_code(q), B, L, cap, heads, hk, d, q.data_ptr(), *q.stride()[:3],
+             k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], lens.data_ptr(), scale,
+             out.data_ptr(), L * heads * d, heads * d, d, ws.data_ptr() if size else None, size)
     return out
