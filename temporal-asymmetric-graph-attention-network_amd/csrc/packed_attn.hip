@@ -306,7 +306,7 @@ struct AttnArgs {
     Div by_g, by_kv, by_splits, by_tiles;   // of the group, the key heads, the splits, a cache's tiles to a sequence
     float c;                          // scale * log2(e)
     float scale;
-    float* part;                      // splits: [split][row of batch][D + 4]
+    float* part;                      // splits: sums [row of the batch][split][D], then (base, total) of each
 };
 
 // One sequence and where its rows lie.  Rows outside every sequence belong to two more that see no key (the run before
@@ -615,15 +615,18 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
     l = half_sum(l);
     if (!R.mine) return;
     if constexpr (SPLIT) {
-        // unnormalised sums with their maximum (in powers of two) and total
-        float* p = A.part + (((int64_t)split * A.n_seq + sq.index) * A.kv_heads + hk) * R.nrows * (D + 4) +
-                   (int64_t)R.row * (D + 4);
+        // unnormalised sums, and behind those of all rows the maxima (in powers of two) and totals; a row's splits together
+        const int64_t at = ((int64_t)sq.index * A.kv_heads + hk) * R.nrows + R.row;
+        float* p = A.part + (at * A.splits + split) * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 store4(p + 32 * d + 2 * i + 4 * half, o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
-        if (half == 0) *(float2*)(p + D) = make_float2(base, l);
+        if (half == 0) {
+            const int64_t all = (int64_t)A.n_seq * A.kv_heads * R.nrows * A.splits;
+            ((float2*)(A.part + all * D))[at * A.splits + split] = make_float2(base, l);
+        }
     } else {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         T* O = (T*)A.out + (int64_t)sq.index * A.os.b + (int64_t)(sq.q0 + R.token) * A.os.tok +
@@ -642,37 +645,41 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
     }
 }
 
-// Joins the splits of a row, a workgroup to a row: the weights of all splits first, then the sums, with the splits dealt
-// out to JG groups of D / 4 lanes whose partial sums are added in order.  At 256 splits a thread has 8 to 32 independent
-// loads instead of a chain of 256.
-constexpr int MAX_SPLITS = 256;
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
-    constexpr int L = D / 4, JG = 256 / L;
-    __shared__ float w[MAX_SPLITS], red[4], tot[4];
-    __shared__ float4 sums[JG][L];
-    const int64_t rows = A.nq * A.G, all = (int64_t)A.n_seq * A.kv_heads * rows, at = blockIdx.x;
-    const int64_t bh = at / rows, row = at - bh * rows, step = all * (D + 4);
-    const float* p = A.part + at * (D + 4);
-    const int s = threadIdx.x, wave = s >> 6;
+// Joins the splits of a row, a workgroup to 32 features of a row and a thread to a split: the weights of all splits first,
+// then the sums, with the splits dealt out to JT / 8 groups of 8 lanes whose partial sums are added in a fixed order.  No
+// thread has more than 8 loads in a row, all independent (a chain over 256 splits took 200 us).
+constexpr int MAX_SPLITS = 512;
+template <typename T, int D, int JT>
+__global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
+    constexpr int JW = JT / 64, JG = JT / 8, CH = D / 32;
+    __shared__ float w[JT], red[JW], tot[JW];
+    __shared__ float4 sums[JW][8];
+    const int rows = (int)A.nq * A.G;
+    const int64_t all = (int64_t)A.n_seq * A.kv_heads * rows, at = blockIdx.x / CH;
+    const int ch = blockIdx.x % CH, s = threadIdx.x, wave = s >> 6, lane = s & 63;
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (s < A.splits) ml = *(const float2*)(p + s * step + D);
+    if (s < A.splits) ml = ((const float2*)(A.part + all * A.splits * D))[at * A.splits + s];
     const bool some = ml.y != 0.f;             // a split without a visible key has no base
     const float m = lane_max<64>(some ? ml.x : -INFINITY);
-    if ((s & 63) == 0) red[wave] = m;
+    if (lane == 0) red[wave] = m;
     __syncthreads();
-    const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float top = red[0];
+#pragma unroll
+    for (int i = 1; i < JW; ++i) top = fmaxf(top, red[i]);
     const float x = some ? __builtin_amdgcn_exp2f(ml.x - top) : 0.f;
     w[s] = x;
     const float t = lane_sum<64>(some ? x * ml.y : 0.f);
-    if ((s & 63) == 0) tot[wave] = t;
+    if (lane == 0) tot[wave] = t;
     __syncthreads();
-    const float l = (tot[0] + tot[1]) + (tot[2] + tot[3]);
-    const int f = s % L, g = s / L;
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < JW; ++i) l += tot[i];
+    const int f = s & 7, g = s >> 3;
+    const float* p = A.part + at * A.splits * D + 32 * ch + 4 * f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int i = g; i < A.splits; i += JG) {
-        const float4 v = *(const float4*)(p + i * step + 4 * f);
+        const float4 v = *(const float4*)(p + (int64_t)i * D);
         const float wi = w[i];
         if (wi != 0.f) {                       // NaN weights too
             o.x = fmaf(v.x, wi, o.x);
@@ -681,19 +688,29 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs A) {
             o.w = fmaf(v.w, wi, o.w);
         }
     }
-    sums[g][f] = o;
-    __syncthreads();
-    if (g != 0 || 4 * f >= A.dim) return;
 #pragma unroll
-    for (int i = 1; i < JG; ++i) {
+    for (int d = 8; d < 64; d <<= 1) {
+        o.x += __shfl_xor(o.x, d, 64);
+        o.y += __shfl_xor(o.y, d, 64);
+        o.z += __shfl_xor(o.z, d, 64);
+        o.w += __shfl_xor(o.w, d, 64);
+    }
+    if (lane < 8) sums[wave][f] = o;
+    __syncthreads();
+    const int feature = 32 * ch + 4 * f;
+    if (s >= 8 || feature >= A.dim) return;
+#pragma unroll
+    for (int i = 1; i < JW; ++i) {
         const float4 v = sums[i][f];
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int64_t b = bh / A.kv_heads, token = row / A.G;
-    const int head = (int)(bh - b * A.kv_heads) * A.G + (int)(row - token * A.G);
-    T* out = (T*)A.out + b * A.os.b + token * A.os.tok + (int64_t)head * A.os.head;
-    store4(out + 4 * f, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const int64_t bh = at / rows;
+    const int row = (int)(at - bh * rows), token = quot(row, A.by_g);
+    const int64_t b = bh / A.kv_heads;
+    const int head = (int)(bh - b * A.kv_heads) * A.G + row - token * A.G;
+    T* out = (T*)A.out + b * A.os.b + (int64_t)token * A.os.tok + (int64_t)head * A.os.head;
+    store4(out + feature, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ
@@ -1174,7 +1191,7 @@ int run_cached(const AttnArgs& A, hipStream_t s) {
     const int64_t rows = A.nq * A.G;
     const bool one = cache_one(rows);
     const int64_t blocks = (int64_t)A.n_seq * A.kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128)) * A.splits;
-    const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows;
+    const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows * (D / 32);
     TAGAN_REQUIRE(blocks <= 0x7fffffff && joins <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
     if (A.splits == 1) {
         if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
@@ -1182,10 +1199,13 @@ int run_cached(const AttnArgs& A, hipStream_t s) {
         TAGAN_CHECK_LAUNCH("cached_attn");
         return TAGAN_OK;
     }
-    if (one) k_attn_fwd<T, D, 1, true, 2><<<(unsigned)blocks, 64, 0, s>>>(A);
+    // 32 keys and values of 128 fp32 features are 32 KB: twice that would leave two waves to a CU
+    if (one) k_attn_fwd<T, D, 1, true, sizeof(T) == 4 && D == 128 ? 1 : 2><<<(unsigned)blocks, 64, 0, s>>>(A);
     else k_attn_fwd<T, D, 4, true, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("cached_attn");
-    k_attn_join<T, D><<<(unsigned)joins, 256, 0, s>>>(A);
+    static_assert(MAX_SPLITS <= 512, "a thread to a split");
+    if (A.splits <= 64) k_attn_join<T, D, 64><<<(unsigned)joins, 64, 0, s>>>(A);
+    else k_attn_join<T, D, 512><<<(unsigned)joins, 512, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("cached_attn (join)");
     return TAGAN_OK;
 }
@@ -1298,7 +1318,7 @@ size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capac
     if (batch <= 0 || new_len <= 0 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
     const int64_t rows = (int64_t)new_len * (heads / kv_heads);
     const int n = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
-    return n == 1 ? 0 : (size_t)n * (size_t)batch * (size_t)(kv_heads * rows) * (size_t)(padded_dim(head_dim) + 4) * 4;
+    return n == 1 ? 0 : (size_t)n * (size_t)batch * (size_t)(kv_heads * rows) * (size_t)(padded_dim(head_dim) + 2) * 4;
 }
 
 int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
