@@ -633,7 +633,8 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * head_dim: multiples of 8 up to 128; heads / kv_heads <= 512; scale > 0.  Pointers and strides (elements) on 16
  * bytes, feature stride 1, token strides of head_dim to 2^21, tokens times heads / kv_heads below 2^31.
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
- * no key is seen.  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
+ * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
+ * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
  * gradients.  workspace: tagan_packed_attn_bwd_workspace bytes.
  * ------------------------------------------------------------------------- */
@@ -641,13 +642,13 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
-                          float* lse, void* stream);
+                          float* lse, void* rest, void* stream);
 size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads);
 int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, const void* out, int64_t o_tok,
-                          int64_t o_head, const float* lse, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
+                          int64_t o_head, const float* lse, const void* rest, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
                           int64_t dq_tok, int64_t dq_head, void* dk, int64_t dk_tok, int64_t dk_head, void* dv,
                           int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream);
 

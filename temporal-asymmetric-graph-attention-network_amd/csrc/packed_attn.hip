@@ -296,13 +296,14 @@ __device__ __forceinline__ int quot(int n, const Div& v) {
 struct AttnArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dq, *dk, *dv;
+    uint16_t* rest;     // bf16 training: out in 32 bits minus out, [nq, heads, dim]
     float* lse;
     float2* stat;       // backward: (log-sum-exp, rowsum(dO O)) of each row
     Strides qs, ks, vs, os, dos, dqs, dks, dvs;
     const int32_t *offs_q, *offs_k;   // packed: [n_seq + 1]; null: a cache
     const int32_t* lens;              // cache: [batch] keys of each
     int64_t nq, nk;                   // packed: tokens in all; cache: new tokens and capacity of each
-    int32_t n_seq, heads, kv_heads, G, dim, causal, splits, ranked;
+    int32_t n_seq, heads, kv_heads, G, dim, causal, splits, ranked, key_blocks;
     Div by_g, by_kv, by_splits, by_tiles;   // of the group, the key heads, the splits, a cache's tiles to a sequence
     float c;                          // scale * log2(e)
     float scale;
@@ -639,6 +640,24 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
                 if (at < A.dim)
                     store4(O + at, o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv);
             }
+        if constexpr (sizeof(T) == 2) {
+            if (A.rest) {
+                uint16_t* rest = A.rest + ((int64_t)(sq.q0 + R.token) * A.heads + hk * A.G + R.g) * A.dim;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int at = 32 * d + 2 * i + 4 * half;
+                        float r[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float x = o[d][i + j] * inv;
+                            r[j] = x - __uint_as_float(f2bf2(x, 0.f) << 16);
+                        }
+                        if (at < A.dim) store4(rest + at, r[0], r[1], r[2], r[3]);
+                    }
+            }
+        }
         // +inf where no key is seen: exp2(s - lse) is 0 in the backward
         if (A.lse && half == 0)
             A.lse[(int64_t)(sq.q0 + R.token) * A.heads + hk * A.G + R.g] = l == 0.f ? INFINITY : base + __log2f(l);
@@ -713,25 +732,53 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
     store4(out + feature, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// ------------------------------------------------------------------------------------------------ backward: dQ
-// Rows as in the forward; also writes (log-sum-exp, delta = rowsum(dO O)) of each row for the key kernel that follows on
-// the stream.
+// ------------------------------------------------------------------------------------------------ backward
+// (log-sum-exp, delta = rowsum(dO O)) of each row, D / 8 lanes to a row.  A short row's dP - delta is a small difference
+// of large terms: delta takes out to 16 bits and more (its bf16 value and the rest that the forward kept).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_attn_stat(AttnArgs A) {
+    constexpr int L = D / 8;
+    const int64_t at = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int x = threadIdx.x % L * 8;
+    if (at >= A.nq * A.heads) return;
+    const int64_t token = at / A.heads, head = at - token * A.heads;
+    float sum = 0.f;
+    if (x < A.dim) {
+        Frag<T> g, o;
+        load_frag(g, (const T*)A.dout + token * A.dos.tok + head * A.dos.head + x);
+        load_frag(o, (const T*)A.o + token * A.os.tok + head * A.os.head + x);
+        sum = dot(g, o);
+        if constexpr (sizeof(T) == 2) {
+            if (A.rest) {
+                load_frag(o, A.rest + at * A.dim + x);
+                sum += dot(g, o);
+            }
+        }
+    }
+    sum = lane_sum<L>(sum);
+    if (x == 0) A.stat[at] = make_float2(A.lse[at], sum);
+}
+
+// Keys of a tile of the dQ blocks: at least as many as the direct loads of all waves bring
+template <typename T, int D, int WAVES>
+constexpr int dq_keys() {
+    constexpr int KT = WAVES == 1 || (D == 128 && sizeof(T) == 4) ? 32 : 64, ALL = Tile<T, D>::RPW * WAVES;
+    return KT > ALL ? KT : ALL;
+}
+
+// dQ: rows as in the forward.
 template <typename T, int D, int WAVES, int STAGES>
-__global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dq(AttnArgs A) {
-    constexpr int KT = WAVES == 1 || (D == 128 && sizeof(T) == 4) ? 32 : 64, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+__device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks, char* ks0, char* ks1, char* vs0, char* vs1) {
+    constexpr int KT = dq_keys<T, D, WAVES>(), NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
-    constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
-    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
-    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads;
+    const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads;
     Seq sq;
-    if (!locate<ROWS>(A, quot(gridDim.x, A.by_kv) - 1 - vt, sq)) return;
+    if (!locate<ROWS>(A, quot(blocks, A.by_kv) - 1 - vt, sq)) return;
     const Rows R = rows_of<ROWS>(A, sq);
     const int kend = R.most;
     const int64_t head = hk * A.G + R.g, tok = sq.q0 + R.token;
     const T* Q = (const T*)A.q + tok * A.qs.tok + head * A.qs.head;
-    const T* O = (const T*)A.o + tok * A.os.tok + head * A.os.head;
     const T* DO = (const T*)A.dout + tok * A.dos.tok + head * A.dos.head;
     const T* K = (const T*)A.k + (int64_t)sq.k0 * A.ks.tok + (int64_t)hk * A.ks.head;
     const T* V = (const T*)A.v + (int64_t)sq.k0 * A.vs.tok + (int64_t)hk * A.vs.head;
@@ -740,24 +787,20 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
     const auto klay = TL::template lay<WAVES>(kstep, bytes), vlay = TL::template lay<WAVES>(vstep, bytes);
 
     Frag<T> qf[NC], gf[NC];
-    float delta = 0.f;
+    float lse = INFINITY, delta = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         qf[c].zero();
         gf[c].zero();
         if (R.mine && 16 * c + 8 * half < A.dim) {
-            Frag<T> of;
             load_frag(qf[c], Q + 16 * c + 8 * half);
             load_frag(gf[c], DO + 16 * c + 8 * half);
-            load_frag(of, O + 16 * c + 8 * half);
-            delta += dot(gf[c], of);
         }
     }
-    delta = half_sum(delta);
-    float lse = INFINITY;
     if (R.mine) {
-        lse = A.lse[tok * A.heads + head];
-        if (half == 0) A.stat[tok * A.heads + head] = make_float2(lse, delta);
+        const float2 stat = A.stat[tok * A.heads + head];
+        lse = stat.x;
+        delta = stat.y;
     }
     f32x16 dq[ND];
 #pragma unroll
@@ -848,20 +891,19 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 2
 // A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
 // those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
 // the block is what bounds the longest block: the first keys of a long causal sequence are seen by every row of the group.
+template <typename T, int D, int WK, int WR>
+constexpr int dkv_rows() {          // rows of a tile: 32 to a row wave, and enough for a chunk to every lane of the loads
+    constexpr int LEAST = 1024 * WK * WR / Tile<T, D>::ROW;
+    return 32 * WR > LEAST ? 32 * WR : LEAST;
+}
 template <typename T, int D, int WK, int WR, int STAGES>
-__global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_dkv(AttnArgs A) {
+__device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0, char* gs0, char* qs1, char* gs1, char* st0,
+                                         char* st1, char* vl) {
     typedef Tile<T, D> TL;
-    // rows of a tile: 32 to a row wave, and enough for a chunk to every lane of the direct loads
-    constexpr int WAVES = WK * WR, NC = D / 16, ND = D / 32, KEYS = 32 * WK;
-    constexpr int LEAST = 1024 * WAVES / TL::ROW, QT = 32 * WR > LEAST ? 32 * WR : LEAST;
-    constexpr int TILE = QT * TL::ROW;
-    // the keys' own v: in LDS where the accumulators and k leave no registers for it
-    constexpr bool VL = D == 128;
-    constexpr int SECOND = STAGES == 2 ? TILE : 16;
-    __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
-    __shared__ __align__(16) char vl[VL ? KEYS * TL::ROW : 16];
+    constexpr int WAVES = WK * WR, NC = D / 16, ND = D / 32, KEYS = 32 * WK, QT = dkv_rows<T, D, WK, WR>(), TILE = QT * TL::ROW;
+    constexpr bool VL = D == 128;   // the keys' own v: in LDS where the accumulators and k leave no registers for it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
-    const int vt = quot(blockIdx.x, A.by_kv), hk = (int)blockIdx.x - vt * A.kv_heads, nk = (int)A.nk;
+    const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads, nk = (int)A.nk;
     int i, tile;
     if (A.ranked) {
         int slq = 0, slk = 0;
@@ -1095,6 +1137,19 @@ __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 
         }
 }
 
+// Both in one launch, the key blocks first: they are the longer ones, and the row blocks fill the CUs that they leave.
+template <typename T, int D, int WK, int WR, int STAGES>
+__global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_bwd(AttnArgs A) {
+    typedef Tile<T, D> TL;
+    constexpr int WAVES = WK * WR, QT = dkv_rows<T, D, WK, WR>(), KT = dq_keys<T, D, WAVES>();
+    constexpr int TILE = (QT > KT ? QT : KT) * TL::ROW, SECOND = STAGES == 2 ? TILE : 16;
+    __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
+    __shared__ __align__(16) char vl[D == 128 ? 32 * WK * TL::ROW : 16];
+    const int block = (int)blockIdx.x;
+    if (block < A.key_blocks) attn_dkv<T, D, WK, WR, STAGES>(A, block, qs0, gs0, qs1, gs1, st0, st1, vl);
+    else attn_dq<T, D, WAVES, STAGES>(A, block - A.key_blocks, (int)gridDim.x - A.key_blocks, qs0, qs1, gs0, gs1);
+}
+
 // ------------------------------------------------------------------------------------------------ launches
 constexpr int MAX_DIM = 128, MAX_GROUP = 512;
 
@@ -1145,34 +1200,33 @@ int run_fwd(const AttnArgs& A, hipStream_t s) {
 }
 
 template <typename T, int D, int WK, int WR, int STAGES>
-int launch_dkv(AttnArgs A, hipStream_t s) {
-    const int64_t blocks = (A.nk / (32 * WK) + A.n_seq + 2) * A.kv_heads;
-    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
-    A.ranked = A.n_seq >= 2 && A.n_seq <= ORDERED && blocks < 16 * 256;
-    k_attn_dkv<T, D, WK, WR, STAGES><<<(unsigned)blocks, 64 * WK * WR, 0, s>>>(A);
-    TAGAN_CHECK_LAUNCH("packed_attn_bwd (dk, dv)");
+int launch_bwd(AttnArgs A, hipStream_t s) {
+    const int64_t keys = A.nk > 0 ? (A.nk / (32 * WK) + A.n_seq + 2) * A.kv_heads : 0;
+    const int64_t rows = A.nq > 0 ? (A.nq * A.G / (32 * WK * WR) + A.n_seq + 2) * A.kv_heads : 0;
+    TAGAN_REQUIRE(keys + rows <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
+    A.ranked = A.n_seq >= 2 && A.n_seq <= ORDERED && keys < 16 * 256;
+    A.key_blocks = (int32_t)keys;
+    k_attn_bwd<T, D, WK, WR, STAGES><<<(unsigned)(keys + rows), 64 * WK * WR, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("packed_attn_bwd");
     return TAGAN_OK;
 }
 
 template <typename T, int D>
 int run_bwd(const AttnArgs& A, hipStream_t s) {
-    const bool one = A.nq * A.G < (int64_t)64 * A.n_seq, kone = A.nk < (int64_t)64 * A.n_seq;
-    const int64_t blocks = (A.nq * A.G / (one ? 32 : 128) + A.n_seq + 2) * A.kv_heads;
-    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
     if (A.nq > 0) {
-        if (one) k_attn_dq<T, D, 1, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
-        else k_attn_dq<T, D, 4, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
-        TAGAN_CHECK_LAUNCH("packed_attn_bwd (dq)");
+        const int64_t blocks = (A.nq * A.heads + 2048 / D - 1) / (2048 / D);
+        TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many rows");
+        k_attn_stat<T, D><<<(unsigned)blocks, 256, 0, s>>>(A);
+        TAGAN_CHECK_LAUNCH("packed_attn_bwd (row sums)");
     }
-    if (A.nk == 0) return TAGAN_OK;
-    const int64_t wide = (A.nk / 128 + A.n_seq + 2) * A.kv_heads;
-    // Two row waves where blocks are few and the longest of them decides, and for 256-byte rows, whose accumulators leave
-    // two waves to a SIMD in any case; with 4 blocks to a CU and more, smaller ones keep the CUs busier (48 histories to
-    // 512 tokens, 64 features: 84 us against 111).  fp32 at 128 features: one wave's registers fill a SIMD.
-    if (kone) return launch_dkv<T, D, 1, 1, 1>(A, s);
-    if constexpr (sizeof(T) == 4 && D == 128) return launch_dkv<T, D, 4, 1, 2>(A, s);
-    else if (wide >= 4 * 256 && D * sizeof(T) < 256) return launch_dkv<T, D, 4, 1, 2>(A, s);
-    else return launch_dkv<T, D, 4, 2, 2>(A, s);
+    // One-wave blocks where a sequence has few rows and keys.  Two row waves where blocks are few and the longest of them
+    // decides, and for 256-byte rows, whose accumulators leave two waves to a SIMD in any case; with 4 blocks to a CU and
+    // more, smaller ones keep the CUs busier (48 histories to 512 tokens, 64 features, dK and dV: 84 us against 111).  fp32
+    // at 128 features: one wave's registers fill a SIMD.
+    if (A.nq * A.G + A.nk < (int64_t)128 * A.n_seq) return launch_bwd<T, D, 1, 1, 1>(A, s);
+    if constexpr (sizeof(T) == 4 && D == 128) return launch_bwd<T, D, 4, 1, 2>(A, s);
+    else if ((A.nk / 128 + A.n_seq + 2) * A.kv_heads >= 4 * 256 && D * sizeof(T) < 256) return launch_bwd<T, D, 4, 1, 2>(A, s);
+    else return launch_bwd<T, D, 4, 2, 2>(A, s);
 }
 
 // Splits of the key axis for a cache: enough one-wave blocks for 16 to a CU, and at least 64 keys of the capacity to
@@ -1223,7 +1277,7 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
-                          float* lse, void* stream) {
+                          float* lse, void* rest, void* stream) {
     int rc = check_shape("packed_attn_fwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
@@ -1234,7 +1288,9 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_fwd: null offsets");
     const int es = dtype == TAGAN_F32 ? 4 : 2;
     AttnArgs A = {};
-    A.q = q; A.k = k; A.v = v; A.out = out; A.lse = lse;
+    A.q = q; A.k = k; A.v = v; A.out = out; A.lse = lse; A.rest = (uint16_t*)rest;
+    TAGAN_REQUIRE(!rest || (dtype == TAGAN_BF16 && ((uintptr_t)rest & 15) == 0), TAGAN_ERR_ARG,
+                  "packed_attn_fwd: rest is of bf16 and lies on 16 bytes");
     A.qs = {0, q_tok, q_head};
     A.ks = {0, k_tok, k_head};
     A.vs = {0, v_tok, v_head};
@@ -1265,7 +1321,7 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, const void* out, int64_t o_tok,
-                          int64_t o_head, const float* lse, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
+                          int64_t o_head, const float* lse, const void* rest, const void* dout, int64_t do_tok, int64_t do_head, void* dq,
                           int64_t dq_tok, int64_t dq_head, void* dk, int64_t dk_tok, int64_t dk_head, void* dv,
                           int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("packed_attn_bwd", dtype, heads, kv_heads, head_dim, scale);
@@ -1282,7 +1338,10 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     AttnArgs A = {};
     A.q = q; A.k = k; A.v = v; A.o = out; A.dout = dout;
     A.dq = dq; A.dk = dk; A.dv = dv;
-    A.lse = (float*)lse; A.stat = (float2*)workspace;
+    A.lse = (float*)lse; A.stat = (float2*)workspace; A.rest = (uint16_t*)rest;
+    TAGAN_REQUIRE(!rest || (dtype == TAGAN_BF16 && ((uintptr_t)rest & 15) == 0), TAGAN_ERR_ARG,
+                  "packed_attn_bwd: rest is of bf16 and lies on 16 bytes");
+    TAGAN_REQUIRE(((uintptr_t)workspace & 7) == 0, TAGAN_ERR_ARG, "packed_attn_bwd: the workspace has to lie on 8 bytes");
     A.qs = {0, q_tok, q_head};
     A.ks = {0, k_tok, k_head};
     A.vs = {0, v_tok, v_head};

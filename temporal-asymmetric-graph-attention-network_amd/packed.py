@@ -253,7 +253,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
 
 # ----------------------------------------------------------------------------- packed attention
 class PackedAttnFn(torch.autograd.Function):
-    """softmax(scale q kᵀ) v inside each packed sequence; saves the output and the rows' log-sum-exp."""
+    """softmax(scale q kᵀ) v inside each packed sequence; saves the output (bf16: with its rounding, 2 bytes more to an
+    element) and the rows' log-sum-exp."""
 
     @staticmethod
     def forward(ctx, q, k, v, offsets, offsets_k, causal: bool, scale: float):
@@ -263,20 +264,21 @@ class PackedAttnFn(torch.autograd.Function):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         needs = any(ctx.needs_input_grad[:3])
         lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if needs else None
+        rest = torch.empty_like(out) if needs and q.dtype is torch.bfloat16 else None
         if n:
             _run("tagan_packed_attn_fwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, q.data_ptr(),
                  *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], offsets.data_ptr(),
                  offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d,
-                 lse.data_ptr() if needs else None)
+                 lse.data_ptr() if needs else None, None if rest is None else rest.data_ptr())
         if needs:
-            ctx.save_for_backward(q, k, v, out, lse, offsets, offsets_k)
+            ctx.save_for_backward(q, k, v, out, lse, rest, offsets, offsets_k)
             ctx.cfg = (causal, scale)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, offsets, offsets_k = ctx.saved_tensors
+        q, k, v, out, lse, rest, offsets, offsets_k = ctx.saved_tensors
         causal, scale = ctx.cfg
         dout = _dense(dout)
         n, heads, d = q.shape
@@ -287,8 +289,8 @@ class PackedAttnFn(torch.autograd.Function):
             ws = torch.empty(max(size, 1), dtype=torch.uint8, device=q.device)
             _run("tagan_packed_attn_bwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, q.data_ptr(),
                  *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], offsets.data_ptr(),
-                 offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d, lse.data_ptr(), dout.data_ptr(),
-                 *dout.stride()[:2], dq.data_ptr(), heads * d, d, dk.data_ptr(), hk * d, d, dv.data_ptr(), hk * d, d,
+                 offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d, lse.data_ptr(),
+                 None if rest is None else rest.data_ptr(), dout.data_ptr(), *dout.stride()[:2], dq.data_ptr(), heads * d, d, dk.data_ptr(), hk * d, d, dv.data_ptr(), hk * d, d,
                  ws.data_ptr(), size)
         return dq, dk, dv, None, None, None, None
 

@@ -138,7 +138,7 @@ A = 0x10000   # a pointer that is never followed
 
 def _fwd(L, dtype=0, n_seq=1, nq=4, nk=4, heads=4, kv=2, d=16, q=A, tok=64, head=16, offs=A, scale=0.25):
     return L.tagan_packed_attn_fwd(dtype, n_seq, nq, nk, heads, kv, d, q, tok, head, A, 32, 16, A, 32, 16, offs, offs,
-                                   1, scale, A, 64, 16, None, None)
+                                   1, scale, A, 64, 16, None, None, None)
 
 
 @pytest.mark.parametrize("kw, status", [
@@ -154,7 +154,7 @@ def test_packed_fwd_entry(kw, status):
 def _bwd(L, ws=A, size=None, lse=A, head=16, heads=4):
     size = L.tagan_packed_attn_bwd_workspace(4, heads) if size is None else size
     return L.tagan_packed_attn_bwd(0, 1, 4, 4, heads, 2, 16, A, 64, head, A, 32, 16, A, 32, 16, A, A, 1, 0.25, A, 64,
-                                   16, lse, A, 64, 16, A, 64, 16, A, 32, 16, A, 32, 16, ws, size, None)
+                                   16, lse, None, A, 64, 16, A, 64, 16, A, 32, 16, A, 32, 16, ws, size, None)
 
 
 @pytest.mark.parametrize("kw, status", [(dict(size=4 * 4 * 8 - 1), -4), (dict(ws=None), -4), (dict(lse=None), -4),
