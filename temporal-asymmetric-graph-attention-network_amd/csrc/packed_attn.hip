@@ -111,11 +111,15 @@ __device__ __forceinline__ void store4(float* p, float a, float b, float c, floa
 template <typename T, int D>
 struct Tile {
     static constexpr int E = 16 / (int)sizeof(T);      // elements of a chunk
-    static constexpr int CPR = D / E;                  // chunks of a row: 4 to 32
+    static constexpr int CPR = D / E;                  // chunks of a row: 2 to 32
     static constexpr int ROW = D * (int)sizeof(T);     // bytes of a row
+    // 16 features: the 32-wide transposed reads pass the row's end (and at the last one the tile's); what they bring from
+    // there goes to accumulator rows that are never stored
+    static constexpr int PAD = D < 32 ? 64 : 0;
 
     __device__ static __forceinline__ int swz(int r) {
-        if constexpr (CPR == 4) return (r >> 2) & 3;
+        if constexpr (CPR == 2) return (r >> 3) & 1;
+        else if constexpr (CPR == 4) return (r >> 2) & 3;
         else if constexpr (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -450,7 +454,8 @@ template <typename T, int D, int WAVES>
 struct Shape {
     // keys of a tile: 64; 32 for one-wave blocks and for 128 features, whose scores then leave the forward three waves to
     // a SIMD (ragged prompts 345 -> 315 us)
-    static constexpr int KT = WAVES == 1 || D == 128 ? 32 : 64;
+    static constexpr int LEAST = WAVES == 1 || D == 128 ? 32 : 64, ALL = Tile<T, D>::RPW * WAVES;
+    static constexpr int KT = LEAST > ALL ? LEAST : ALL;   // a wave load at least to every wave
 };
 
 // A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
@@ -458,12 +463,12 @@ struct Shape {
 // many more blocks of a CU hide each other's waits.
 template <typename T, int D, int WAVES, bool SPLIT, int STAGES>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3) k_attn_fwd(AttnArgs A) {
-    constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     // two buffers, each an object of its own: reads of one do not wait for the loads of the other
-    constexpr int SECOND = STAGES == 2 ? KT * TL::ROW : 16;
-    __shared__ __align__(16) char ks0[KT * TL::ROW], ks1[SECOND];
-    __shared__ __align__(16) char vs0[KT * TL::ROW], vs1[SECOND];
+    constexpr int SECOND = STAGES == 2 ? KT * TL::ROW + TL::PAD : 16;
+    __shared__ __align__(16) char ks0[KT * TL::ROW + TL::PAD], ks1[SECOND];
+    __shared__ __align__(16) char vs0[KT * TL::ROW + TL::PAD], vs1[SECOND];
     const int lane = threadIdx.x & 63, half = lane >> 5;
     int bid = blockIdx.x, split = 0, tiles = quot(gridDim.x, A.by_kv);
     if constexpr (SPLIT) {
@@ -769,7 +774,7 @@ constexpr int dq_keys() {
 // dQ: rows as in the forward.
 template <typename T, int D, int WAVES, int STAGES>
 __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks, char* ks0, char* ks1, char* vs0, char* vs1) {
-    constexpr int KT = dq_keys<T, D, WAVES>(), NB = KT / 32, NC = D / 16, ND = D / 32, ROWS = 32 * WAVES;
+    constexpr int KT = dq_keys<T, D, WAVES>(), NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads;
@@ -900,7 +905,7 @@ template <typename T, int D, int WK, int WR, int STAGES>
 __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0, char* gs0, char* qs1, char* gs1, char* st0,
                                          char* st1, char* vl) {
     typedef Tile<T, D> TL;
-    constexpr int WAVES = WK * WR, NC = D / 16, ND = D / 32, KEYS = 32 * WK, QT = dkv_rows<T, D, WK, WR>(), TILE = QT * TL::ROW;
+    constexpr int WAVES = WK * WR, NC = D / 16, ND = (D + 31) / 32, KEYS = 32 * WK, QT = dkv_rows<T, D, WK, WR>(), TILE = QT * TL::ROW;
     constexpr bool VL = D == 128;   // the keys' own v: in LDS where the accumulators and k leave no registers for it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
     const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads, nk = (int)A.nk;
@@ -1142,7 +1147,7 @@ template <typename T, int D, int WK, int WR, int STAGES>
 __global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_bwd(AttnArgs A) {
     typedef Tile<T, D> TL;
     constexpr int WAVES = WK * WR, QT = dkv_rows<T, D, WK, WR>(), KT = dq_keys<T, D, WAVES>();
-    constexpr int TILE = (QT > KT ? QT : KT) * TL::ROW, SECOND = STAGES == 2 ? TILE : 16;
+    constexpr int TILE = (QT > KT ? QT : KT) * TL::ROW + TL::PAD, SECOND = STAGES == 2 ? TILE : 16;
     __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
     __shared__ __align__(16) char vl[D == 128 ? 32 * WK * TL::ROW : 16];
     const int block = (int)blockIdx.x;
@@ -1185,6 +1190,8 @@ int check_tensor(const char* what, const char* name, const void* p, Strides& s, 
 
 #define TAGAN_BY_DIM(T, dim, F)                                    \
     ((dim) <= 32 ? F<T, 32> : (dim) <= 64 ? F<T, 64> : F<T, 128>)
+// with a tile of its own for the framework's 16 features, half the products of 32
+#define TAGAN_BY_DIM16(T, dim, F) ((dim) <= 16 ? F<T, 16> : TAGAN_BY_DIM(T, dim, F))
 
 template <typename T, int D>
 int run_fwd(const AttnArgs& A, hipStream_t s) {
@@ -1309,8 +1316,8 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     hipStream_t s = as_stream(stream);
-    return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_fwd)(A, s)
-                              : TAGAN_BY_DIM(uint16_t, head_dim, run_fwd)(A, s);
+    return dtype == TAGAN_F32 ? TAGAN_BY_DIM16(float, head_dim, run_fwd)(A, s)
+                              : TAGAN_BY_DIM16(uint16_t, head_dim, run_fwd)(A, s);
 }
 
 size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads) {
@@ -1368,8 +1375,8 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     TAGAN_REQUIRE((A.qs.head > A.dos.head ? A.qs.head : A.dos.head) * A.G * es < (1ll << 30), TAGAN_ERR_UNSUPPORTED,
                   "packed_attn_bwd: head strides %lld and %lld", (long long)q_head, (long long)do_head);
     hipStream_t s = as_stream(stream);
-    return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_bwd)(A, s)
-                              : TAGAN_BY_DIM(uint16_t, head_dim, run_bwd)(A, s);
+    return dtype == TAGAN_F32 ? TAGAN_BY_DIM16(float, head_dim, run_bwd)(A, s)
+                              : TAGAN_BY_DIM16(uint16_t, head_dim, run_bwd)(A, s);
 }
 
 size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
