@@ -328,20 +328,30 @@ __device__ __forceinline__ int edge(const int32_t* offs, int n_seq, int n, int i
     return max(0, min(n, offs[i - 1]));
 }
 
-// The sequence of virtual tile vt: sequence i starts at floor(edge_i * mul / tile) + i, which leaves each room for
-// ceil(length * mul / tile) tiles.  64 probes to a step of the search.
-__device__ __forceinline__ int find_seq(const int32_t* offs, int n_seq, int n, int mul, int tile, int vt) {
-    int lo = 0, count = n_seq + 2;
-    while (count > 1) {
+// The sequence of virtual tile vt, its first token and its length: sequence i starts at floor(edge_i * mul / tile) + i,
+// which leaves each room for ceil(length * mul / tile) tiles.  64 probes to a step of the search; the last step's probes
+// are neighbours and hold both edges.
+struct Found {
+    int i, begin, length, start;
+};
+__device__ __forceinline__ Found find_seq(const int32_t* offs, int n_seq, int n, int mul, int tile, int vt) {
+    int lo = 0, count = n_seq + 2, hit, e;
+    for (;;) {
         const int step = (count + 63) / 64;
         const int i = lo + (int)(threadIdx.x & 63) * step;
-        const bool at = i < lo + count && edge(offs, n_seq, n, i) * mul / tile + i <= vt;
-        const int hit = __popcll(__ballot(at));
-        const int next = lo + (hit > 0 ? hit - 1 : 0) * step;
-        count = min(step, lo + count - next);
-        lo = next;
+        e = edge(offs, n_seq, n, min(i, n_seq + 2));
+        hit = max(1, (int)__popcll(__ballot(i < lo + count && e * mul / tile + i <= vt)));
+        if (step == 1) break;
+        count = min(step, count - (hit - 1) * step);
+        lo += (hit - 1) * step;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    Found f;
+    f.i = __builtin_amdgcn_readfirstlane(lo + hit - 1);
+    f.begin = __builtin_amdgcn_readlane(e, hit - 1);
+    const int end = hit < 64 ? __builtin_amdgcn_readlane(e, hit & 63) : edge(offs, n_seq, n, f.i + 1);
+    f.length = __builtin_amdgcn_readfirstlane(end) - f.begin;
+    f.start = f.begin * mul / tile + f.i;
+    return f;
 }
 
 // Heaviest tiles first.  With up to 62 sequences (and the two runs outside them) a lane keeps one of them, and every
@@ -405,17 +415,22 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
         s.lk = max(0, min((int)A.nk, A.lens[s.index]));
         return true;
     }
-    const int nq = (int)A.nq, i = find_seq(A.offs_q, A.n_seq, nq, A.G, ROWS, vt);
-    s.tile = vt - (edge(A.offs_q, A.n_seq, nq, i) * A.G / ROWS + i);
-    s.q0 = edge(A.offs_q, A.n_seq, nq, i);
-    s.lq = edge(A.offs_q, A.n_seq, nq, i + 1) - s.q0;
-    if (s.lq <= 0 || s.tile * ROWS >= s.lq * A.G) return false;
+    const Found f = find_seq(A.offs_q, A.n_seq, (int)A.nq, A.G, ROWS, vt);
+    s.q0 = f.begin;
+    s.lq = f.length;
+    s.tile = vt - f.start;
+    if (s.lq <= 0 || s.tile < 0 || s.tile * ROWS >= s.lq * A.G) return false;   // below 0: offsets that descend
     s.index = 0;
     s.k0 = 0;
     s.lk = 0;
-    if (i >= 1 && i <= A.n_seq) {
-        s.k0 = edge(A.offs_k, A.n_seq, (int)A.nk, i);
-        s.lk = max(0, edge(A.offs_k, A.n_seq, (int)A.nk, i + 1) - s.k0);
+    if (f.i >= 1 && f.i <= A.n_seq) {
+        if (A.offs_k == A.offs_q && A.nk == A.nq) {
+            s.k0 = f.begin;
+            s.lk = f.length;
+        } else {
+            s.k0 = edge(A.offs_k, A.n_seq, (int)A.nk, f.i);
+            s.lk = max(0, edge(A.offs_k, A.n_seq, (int)A.nk, f.i + 1) - s.k0);
+        }
     }
     return true;
 }
@@ -909,7 +924,7 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
     constexpr bool VL = D == 128;   // the keys' own v: in LDS where the accumulators and k leave no registers for it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
     const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads, nk = (int)A.nk;
-    int i, tile;
+    int i, tile, k0, lk;
     if (A.ranked) {
         int slq = 0, slk = 0;
         if (lane < A.n_seq + 2) {
@@ -927,16 +942,22 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
             return !A.causal ? tiles : span < 0 ? 0 : min(tiles, span / KEYS + 1);
         }, i, tile);
         if (!found) return;
+        k0 = edge(A.offs_k, A.n_seq, nk, i);
+        lk = edge(A.offs_k, A.n_seq, nk, i + 1) - k0;
     } else {
-        i = find_seq(A.offs_k, A.n_seq, nk, 1, KEYS, vt);
-        tile = vt - (edge(A.offs_k, A.n_seq, nk, i) / KEYS + i);
+        const Found f = find_seq(A.offs_k, A.n_seq, nk, 1, KEYS, vt);
+        i = f.i;
+        tile = vt - f.start;
+        k0 = f.begin;
+        lk = f.length;
     }
-    const int k0 = edge(A.offs_k, A.n_seq, nk, i), lk = edge(A.offs_k, A.n_seq, nk, i + 1) - k0, key0 = tile * KEYS;
-    if (lk <= 0 || key0 >= lk) return;
+    const int key0 = tile * KEYS;
+    if (lk <= 0 || tile < 0 || key0 >= lk) return;   // below 0: offsets that descend
     int q0 = 0, lq = 0;
     if (i >= 1 && i <= A.n_seq) {
-        q0 = edge(A.offs_q, A.n_seq, (int)A.nq, i);
-        lq = max(0, edge(A.offs_q, A.n_seq, (int)A.nq, i + 1) - q0);
+        const bool same = A.offs_k == A.offs_q && A.nk == A.nq;
+        q0 = same ? k0 : edge(A.offs_q, A.n_seq, (int)A.nq, i);
+        lq = same ? lk : max(0, edge(A.offs_q, A.n_seq, (int)A.nq, i + 1) - q0);
     }
     const int G = A.G, past = lk - lq, key = key0 + wk * 32 + (lane & 31);
     const bool mine = key < lk;
@@ -953,10 +974,6 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
             if constexpr (!VL) load_frag(vf[c], V + 16 * c + 8 * half);
         }
     }
-    if constexpr (VL)
-        TL::template fill<KEYS, WAVES>(vl, (const T*)A.v + (int64_t)(k0 + key0) * A.vs.tok + (int64_t)hk * A.vs.head,
-                                       (uint32_t)(A.vs.tok * sizeof(T)), min(KEYS, lk - key0), bytes,
-                                       TL::template lay<WAVES>((uint32_t)(A.vs.tok * sizeof(T)), bytes));
     f32x16 dk[ND], dv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -1066,6 +1083,12 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
             }
         }
     };
+    if constexpr (VL) {
+        if (ntiles > 0)
+            TL::template fill<KEYS, WAVES>(vl, (const T*)A.v + (int64_t)(k0 + key0) * A.vs.tok + (int64_t)hk * A.vs.head,
+                                       (uint32_t)(A.vs.tok * sizeof(T)), min(KEYS, lk - key0), bytes,
+                                       TL::template lay<WAVES>((uint32_t)(A.vs.tok * sizeof(T)), bytes));
+    }
     const auto rows = [&](char* qs, char* gs, const char* st, int n) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < QT; q += 32 * WR) part(qs, gs, st, n, q + 32 * wr);
@@ -1142,9 +1165,14 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
         }
 }
 
+// waves to a SIMD that the accumulators and k, v leave room for
+template <typename T, int D, int WK>
+constexpr int bwd_waves() {
+    return D * sizeof(T) == 512 ? 1 : D == 16 && WK == 1 ? 4 : 2;
+}
 // Both in one launch, the key blocks first: they are the longer ones, and the row blocks fill the CUs that they leave.
 template <typename T, int D, int WK, int WR, int STAGES>
-__global__ void __launch_bounds__(WK* WR * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) k_attn_bwd(AttnArgs A) {
+__global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_bwd(AttnArgs A) {
     typedef Tile<T, D> TL;
     constexpr int WAVES = WK * WR, QT = dkv_rows<T, D, WK, WR>(), KT = dq_keys<T, D, WAVES>();
     constexpr int TILE = (QT > KT ? QT : KT) * TL::ROW + TL::PAD, SECOND = STAGES == 2 ? TILE : 16;
@@ -1193,13 +1221,16 @@ int check_tensor(const char* what, const char* name, const void* p, Strides& s, 
 // with a tile of its own for the framework's 16 features, half the products of 32
 #define TAGAN_BY_DIM16(T, dim, F) ((dim) <= 16 ? F<T, 16> : TAGAN_BY_DIM(T, dim, F))
 
+// a launch counts its threads in 32 bits
+bool fits_grid(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads && blocks <= 0x7fffffff; }
+
 template <typename T, int D>
 int run_fwd(const AttnArgs& A, hipStream_t s) {
     // waves to a block by the rows that a sequence has on average: 32-row blocks where four waves would mostly idle
     const bool one = A.nq * A.G < (int64_t)64 * A.n_seq;
     const int rows = one ? 32 : 128;
     const int64_t blocks = (A.nq * A.G / rows + A.n_seq + 2) * A.kv_heads;
-    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
+    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256), TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
     if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
     else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("packed_attn_fwd");
@@ -1210,7 +1241,7 @@ template <typename T, int D, int WK, int WR, int STAGES>
 int launch_bwd(AttnArgs A, hipStream_t s) {
     const int64_t keys = A.nk > 0 ? (A.nk / (32 * WK) + A.n_seq + 2) * A.kv_heads : 0;
     const int64_t rows = A.nq > 0 ? (A.nq * A.G / (32 * WK * WR) + A.n_seq + 2) * A.kv_heads : 0;
-    TAGAN_REQUIRE(keys + rows <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
+    TAGAN_REQUIRE(fits_grid(keys + rows, 64 * WK * WR), TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
     A.ranked = A.n_seq >= 2 && A.n_seq <= ORDERED && keys < 16 * 256;
     A.key_blocks = (int32_t)keys;
     k_attn_bwd<T, D, WK, WR, STAGES><<<(unsigned)(keys + rows), 64 * WK * WR, 0, s>>>(A);
@@ -1222,7 +1253,7 @@ template <typename T, int D>
 int run_bwd(const AttnArgs& A, hipStream_t s) {
     if (A.nq > 0) {
         const int64_t blocks = (A.nq * A.heads + 2048 / D - 1) / (2048 / D);
-        TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many rows");
+        TAGAN_REQUIRE(fits_grid(blocks, 256), TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many rows");
         k_attn_stat<T, D><<<(unsigned)blocks, 256, 0, s>>>(A);
         TAGAN_CHECK_LAUNCH("packed_attn_bwd (row sums)");
     }
@@ -1253,7 +1284,8 @@ int run_cached(const AttnArgs& A, hipStream_t s) {
     const bool one = cache_one(rows);
     const int64_t blocks = (int64_t)A.n_seq * A.kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128)) * A.splits;
     const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows * (D / 32);
-    TAGAN_REQUIRE(blocks <= 0x7fffffff && joins <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
+    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256) && fits_grid(joins, 512), TAGAN_ERR_UNSUPPORTED,
+                  "cached_attn: too many rows");
     if (A.splits == 1) {
         if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
         else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);

@@ -177,7 +177,8 @@ int run_rotary(const RotArgs& A, hipStream_t s, const char* what) {
     // few tokens spread over as many CUs)
     const bool four = A.tokens >= 4 * 2048;
     const int64_t blocks = four ? (A.tokens + 3) / 4 : A.tokens;
-    TAGAN_REQUIRE(blocks <= 0x7fffffff, TAGAN_ERR_UNSUPPORTED, "%s: %lld tokens", what, (long long)A.tokens);
+    TAGAN_REQUIRE(blocks <= 0xffffffffll / RB, TAGAN_ERR_UNSUPPORTED,   // a launch counts its threads in 32 bits
+                  "%s: %lld tokens", what, (long long)A.tokens);
     if (vec_ok(A, (int)sizeof(S))) {
         if (four) k_rotary<S, true, 4><<<(unsigned)blocks, RB, 0, s>>>(A);
         else k_rotary<S, true, 1><<<(unsigned)blocks, RB, 0, s>>>(A);
