@@ -116,37 +116,52 @@ __global__ void __launch_bounds__(RB) k_rotary(RotArgs A) {
             else if constexpr (VEC) { at = item * E; second = at; pair = at / 2; }
             else { at = 2 * item; second = at + 1; pair = item; }
             const float2* w = cs + t * half + pair;
-            for (int h = threadIdx.x / items; h < X.heads; h += step) {
-                const S* src = in + h * X.ih;
-                S* dst = out + h * X.oh;
-                if constexpr (VEC) {
-                    const uint4 u = *(const uint4*)(src + at);
-                    if (second < 0) {
-                        *(uint4*)(dst + at) = u;
-                    } else if (!A.interleaved) {
-                        float x[E], y[E];
-                        unpack<S>(u, x);
-                        unpack<S>(*(const uint4*)(src + second), y);
+            if constexpr (VEC) {
+                // U heads at a time, all loads before the first store (outputs may be the inputs, so the compiler keeps
+                // their order): 117 -> 97 us for 24001 tokens of 40 heads
+                constexpr int U = 4;
+                for (int h0 = threadIdx.x / items; h0 < X.heads; h0 += U * step) {
+                    uint4 a[U], b[U];
 #pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const float c = w[e].x, s = w[e].y, xv = x[e], yv = y[e];
-                            x[e] = xv * c - yv * s;
-                            y[e] = xv * s + yv * c;
+                    for (int j = 0; j < U; ++j) {
+                        const int h = min(h0 + j * step, X.heads - 1);
+                        a[j] = *(const uint4*)(in + h * X.ih + at);
+                        if (second > at) b[j] = *(const uint4*)(in + h * X.ih + second);
+                    }
+#pragma unroll
+                    for (int j = 0; j < U; ++j) {
+                        if (h0 + j * step >= X.heads) break;
+                        S* dst = out + (h0 + j * step) * X.oh;
+                        if (second < 0) {
+                            *(uint4*)(dst + at) = a[j];
+                            continue;
                         }
-                        *(uint4*)(dst + at) = pack<S>(x);
-                        *(uint4*)(dst + second) = pack<S>(y);
-                    } else {
-                        float x[E];
-                        unpack<S>(u, x);
+                        float x[E], y[E];
+                        unpack<S>(a[j], x);
+                        if (!A.interleaved) {
+                            unpack<S>(b[j], y);
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float c = w[e / 2].x, s = w[e / 2].y, xv = x[e], yv = x[e + 1];
-                            x[e] = xv * c - yv * s;
-                            x[e + 1] = xv * s + yv * c;
+                            for (int e = 0; e < E; ++e) {
+                                const float c = w[e].x, s = w[e].y, xv = x[e], yv = y[e];
+                                x[e] = xv * c - yv * s;
+                                y[e] = xv * s + yv * c;
+                            }
+                            *(uint4*)(dst + second) = pack<S>(y);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < E; e += 2) {
+                                const float c = w[e / 2].x, s = w[e / 2].y, xv = x[e], yv = x[e + 1];
+                                x[e] = xv * c - yv * s;
+                                x[e + 1] = xv * s + yv * c;
+                            }
                         }
                         *(uint4*)(dst + at) = pack<S>(x);
                     }
-                } else {
+                }
+            } else {
+                for (int h = threadIdx.x / items; h < X.heads; h += step) {
+                    const S* src = in + h * X.ih;
+                    S* dst = out + h * X.oh;
                     if (second < 0) {
                         dst[at] = src[at];
                     } else {
