@@ -20,7 +20,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._lib import check, dtype_code, lib, require_hip
 
@@ -161,26 +160,25 @@ def _turn(q, k, positions, inv_freq, interleaved, scale, inverse):
 
 
 class RotaryFn(torch.autograd.Function):
-    """(q, k) turned by their positions; the gradient is turned back."""
+    """(q, k) turned by their positions, or back; the gradient is the other turn, of any order."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved: bool, scale: float):
+    def forward(ctx, q, k, positions, inv_freq, interleaved: bool, scale: float, inverse: int):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.cfg = (interleaved, scale)
+        ctx.cfg = (interleaved, scale, 1 - inverse)
         ctx.set_materialize_grads(False)
-        return _turn(q, k, positions, inv_freq, interleaved, scale, 0)
+        return _turn(q, k, positions, inv_freq, interleaved, scale, inverse)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         if dq is None and dk is None:
-            return (None,) * 6
+            return (None,) * 7
         if dq is None:
-            dk, _ = _turn(dk, None, positions, inv_freq, *ctx.cfg, 1)
+            dk, _ = RotaryFn.apply(dk, None, positions, inv_freq, *ctx.cfg)
         else:
-            dq, dk = _turn(dq, dk, positions, inv_freq, *ctx.cfg, 1)
-        return dq, dk, None, None, None, None
+            dq, dk = RotaryFn.apply(dq, dk, positions, inv_freq, *ctx.cfg)
+        return dq, dk, None, None, None, None, None
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -188,7 +186,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """q [N, heads, d] and k [N, kv_heads, d] (or None) turned by ``positions`` [N] (int32, int64, float32 or float64:
     indices or event times) times ``inv_freq`` [r / 2]: the first r features of each head in pairs (i, i + r/2), or
     (2i, 2i + 1) with ``interleaved``, times ``scale``; the features behind them are copied.  Angles are formed in
-    fp64.  Gradients flow to q and k."""
+    fp64.  Gradients flow to q and k (not to positions)."""
     _storage(q, k)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         _refuse("q and k: %s", _shapes(q, k))
@@ -202,7 +200,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         _refuse("scale %g", scale)
     inv_freq = _frequencies(inv_freq, q.shape[2])
     _on_device(q, k, positions, inv_freq)
-    return RotaryFn.apply(q, k, positions.contiguous(), inv_freq, bool(interleaved), float(scale))
+    return RotaryFn.apply(q, k, positions.contiguous(), inv_freq, bool(interleaved), float(scale), 0)
 
 
 def _cache(t: torch.Tensor, name: str) -> None:
@@ -276,8 +274,9 @@ class PackedAttnFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():      # create_graph: the gradients would pass as constants
+            raise RuntimeError("packed.attention has no second derivative")
         q, k, v, out, lse, rest, offsets, offsets_k = ctx.saved_tensors
         causal, scale = ctx.cfg
         dout = _dense(dout)
@@ -316,7 +315,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     Queries that see no key (an empty history, or Lq > Lk with ``causal``) and tokens outside every history (before
     the first offset, behind the last) give zeros and get zero gradients; offsets beyond the token count are taken as
     the token count.  What a query does not see, infinities and NaN included, does not reach its output.  Gradients
-    flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.
+    flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.  There is
+    no second derivative (``create_graph`` raises).
     """
     _storage(q, k, v)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:

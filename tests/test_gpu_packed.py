@@ -303,6 +303,88 @@ def test_same_bits_again_and_on_another_stream(dtype):
     assert all(torch.equal(x, y) for x, y in zip(grads, grads2))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_groups_wider_than_a_tile(dtype, d):
+    """A token's rows take several tiles of the key blocks, the last one part empty; short sequences too."""
+    _attend([9, 2], [14, 2], 100, 1, d, dtype)
+    _attend([1, 0, 1, 2] * 10, [1, 0, 1, 2] * 10, 40, 1, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_sequences_than_a_wave_ranks(dtype):
+    lens = [60 + (37 * i) % 80 for i in range(75)]
+    _attend(lens, lens, 2, 1, 16, dtype)
+    _attend(lens[:62], lens[:62], 2, 1, 64, dtype)
+    _attend(lens[:63], lens[:63], 2, 1, 64, dtype, causal=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_sequence_of_a_hundred_thousand(dtype):
+    """Some rows of a sequence whose scores would not fit anywhere."""
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    n, d = 100003, 16
+    q, k, v, do = (_randn(gen, n, 1, d, dtype=dtype) for _ in range(4))
+    v.requires_grad_(True)
+    do[: n - 40] = 0                          # the last rows alone give dv
+    offs = _offs([n])
+    out = packed.attention(q, k, v, offs)
+    dv, = torch.autograd.grad(out, v, do)
+    want = torch.zeros(n, 1, d, dtype=F64, device=DEV)
+    tol = torch.zeros_like(want)
+    for i in (0, 1, 777, 50000, n - 40, n - 1):
+        r = _one(q[i:i + 1].double(), k[:i + 1, 0].double(), v.detach()[:i + 1, 0].double(), True, d ** -0.5, dtype=dtype)
+        _check(out.detach()[i], r["o"], r["to"], "row %d" % i)
+    r = _one(q[n - 40:].double(), k[:, 0].double(), v.detach()[:, 0].double(), True, d ** -0.5, do[n - 40:].double(), dtype)
+    want[:, 0], tol[:, 0] = r["dv"], r["tdv"]
+    _check(dv, want, tol, "dv")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_broadcast_and_head_major_inputs(dtype):
+    """One key head seen as four, heads outermost, k and v of other strides, and a gradient for v alone."""
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    n, d = 90, 32
+    offs = _offs([50, 40])
+    q, do = (_randn(gen, n, 4, d, dtype=dtype) for _ in range(2))
+    k1, v1 = (_randn(gen, n, 1, d, dtype=dtype).requires_grad_(True) for _ in range(2))
+    out = packed.attention(q, k1.expand(-1, 4, -1), v1.expand(-1, 4, -1), offs)
+    grads = torch.autograd.grad(out, (k1, v1), do)
+    k4, v4 = (t.detach().expand(-1, 4, -1).contiguous().requires_grad_(True) for t in (k1, v1))
+    out4 = packed.attention(q, k4, v4, offs)
+    assert torch.equal(out, out4)
+    for g, g4 in zip(grads, torch.autograd.grad(out4, (k4, v4), do)):
+        assert torch.equal(g, g4.sum(1, keepdim=True))      # the expansion's own sum
+    ref = [torch.autograd.grad(packed.attention(a, k4, v4, offs), (a, k4, v4), do)
+           for a in (q.detach().requires_grad_(True),)][0]
+    major = [t.detach().transpose(0, 1).contiguous().transpose(0, 1).requires_grad_(True) for t in (q, k4)]
+    got = torch.autograd.grad(packed.attention(*major, v4, offs), (*major, v4),
+                              do.transpose(0, 1).contiguous().transpose(0, 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    alone, = torch.autograd.grad(packed.attention(q, k4.detach(), v4, offs), v4, do)
+    assert torch.equal(alone, ref[2])
+
+
+def test_no_second_derivative():
+    q = torch.randn(5, 1, 8, device=DEV, requires_grad=True)
+    out = packed.attention(q, q, q, _offs([5]))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), q, create_graph=True)
+
+
+def test_second_derivative_of_a_turn():
+    """The turn is linear: the gradient of a gradient's square is twice the scale's square times the weights."""
+    q = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    w = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    freq, _ = packed.rotary_frequencies(8, device=DEV)
+    out, _ = packed.rotary(q, None, torch.arange(5, device=DEV), freq, scale=1.5)
+    g, = torch.autograd.grad((out * w).sum(), q, create_graph=True)
+    h, = torch.autograd.grad((g * g).sum(), w)
+    # two turns of 12 W of a pair's sum each, and the factors
+    bound = 2 * 1.5 * 1.5 * 40 * W * w.detach().double().abs().sum(-1, keepdim=True)
+    _check(h, 2 * 1.5 ** 2 * w.detach().double(), bound.expand_as(h), "second derivative")
+
+
 # ----------------------------------------------------------------------------- rotary
 def _turned(x, pos, freq, interleaved, scale, sign=1.0):
     r = 2 * freq.numel()
@@ -425,6 +507,51 @@ def test_cached_attention_long_and_wide(dtype):
     _cached(3, 5, 30, [2, 5, 30], 64, 1, 16, dtype)       # fewer rows than new tokens: the first see nothing
     _cached(2, 1, 50, [99, -4], 4, 2, 32, dtype)          # outside the capacity
     _cached(300, 1, 70, [(7 * i) % 71 for i in range(300)], 2, 1, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_caches_with_heads_outermost_and_slices(dtype):
+    """[B, heads, capacity, d] caches seen as [B, capacity, heads, d], and a slice of the batch and of the capacity."""
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    B, cap, hk, d = 3, 200, 2, 64
+    q, k, v = (_randn(gen, B, 2, h, d, dtype=dtype) for h in (4, hk, hk))
+    dense = [_randn(gen, B, cap, hk, d, dtype=dtype) for _ in range(2)]
+    lens = torch.tensor([0, 77, 198], dtype=torch.int32, device=DEV)
+    freq, _ = packed.rotary_frequencies(d, device=DEV)
+    major = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in dense]
+    wide = [torch.zeros(B + 2, cap + 50, hk, d, dtype=dtype, device=DEV) for _ in range(2)]
+    for w, t in zip(wide, dense):
+        w[1:B + 1, 20:20 + cap] = t
+    parts = [w[1:B + 1, 20:20 + cap] for w in wide]
+    res = []
+    for kc, vc in (dense, major, parts):
+        qn = packed.rotary_append(q, k, v, kc, vc, lens, freq)
+        res.append((qn, kc, vc, packed.cached_attention(qn, kc, vc, lens + 2)))
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+    for w in wide:
+        assert not bool(w[0].any()) and not bool(w[-1].any()) and not bool(w[:, :20].any()) and not bool(w[:, 220:].any())
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        flat = torch.zeros(B * cap * hk * d + 1, dtype=dtype, device=DEV)[1:].view(B, cap, hk, d)
+        packed.cached_attention(q, flat, flat, lens)
+
+
+def test_two_calls_at_once():
+    """The same operators on two streams with nothing between them: each has its own workspace."""
+    gen = torch.Generator(device=DEV).manual_seed(15)
+    q = [_randn(gen, 4, 1, 8, 64, dtype=torch.bfloat16) for _ in range(2)]
+    caches = [[_randn(gen, 4, 3000, 2, 64, dtype=torch.bfloat16) for _ in range(2)] for _ in range(2)]
+    lens = torch.tensor([3000, 1, 1500, 64], dtype=torch.int32, device=DEV)
+    want = [packed.cached_attention(a, *c, lens) for a, c in zip(q, caches)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(packed.cached_attention(q[i], *caches[i], lens))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
 
 
 def test_cached_attention_empty():
