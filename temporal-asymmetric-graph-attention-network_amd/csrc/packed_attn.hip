@@ -611,8 +611,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
             tiles_ready();
             tile(ks0, vs0, kt);
         }
-    }
-    else {
+    } else {
         if (kbeg < kend) load(ks0, vs0, kbeg);
         for (int kt = kbeg; kt < kend; kt += 2 * KT) {
             tiles_ready();                              // and every wave is done with the other buffer
@@ -797,7 +796,8 @@ constexpr int dq_keys() {
 
 // dQ: rows as in the forward.
 template <typename T, int D, int WAVES, int STAGES>
-__device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks, char* ks0, char* ks1, char* vs0, char* vs1) {
+__device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks, char* ks0, char* ks1, char* vs0,
+                                        char* vs1) {
     constexpr int KT = dq_keys<T, D, WAVES>(), NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
     const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -890,8 +890,7 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
             tiles_ready();
             tile(ks0, vs0, kt);
         }
-    }
-    else {
+    } else {
         if (kend > 0) load(ks0, vs0, 0);
         for (int kt = 0; kt < kend; kt += 2 * KT) {
             tiles_ready();
@@ -917,8 +916,8 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
-// dK, dV.  A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the rows that see
-// those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
+// dK, dV.  A wave has 32 keys (in its lanes); WK waves side by side have the block's keys and WR of them share the
+// rows that see those keys, 32 rows of every tile to each.  The WR partial sums are added in LDS, in order.  Splitting the rows inside
 // the block is what bounds the longest block: the first keys of a long causal sequence are seen by every row of the group.
 template <typename T, int D, int WK, int WR>
 constexpr int dkv_rows() {          // rows of a tile: 32 to a row wave, and enough for a chunk to every lane of the loads
@@ -926,10 +925,11 @@ constexpr int dkv_rows() {          // rows of a tile: 32 to a row wave, and eno
     return 32 * WR > LEAST ? 32 * WR : LEAST;
 }
 template <typename T, int D, int WK, int WR, int STAGES>
-__device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0, char* gs0, char* qs1, char* gs1, char* st0,
-                                         char* st1, char* vl) {
+__device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0, char* gs0, char* qs1, char* gs1,
+                                         char* st0, char* st1, char* vl) {
     typedef Tile<T, D> TL;
-    constexpr int WAVES = WK * WR, NC = D / 16, ND = (D + 31) / 32, KEYS = 32 * WK, QT = dkv_rows<T, D, WK, WR>(), TILE = QT * TL::ROW;
+    constexpr int WAVES = WK * WR, NC = D / 16, ND = (D + 31) / 32, KEYS = 32 * WK;
+    constexpr int QT = dkv_rows<T, D, WK, WR>(), TILE = QT * TL::ROW;
     constexpr bool VL = D == 128;   // the keys' own v: in LDS where the accumulators and k leave no registers for it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, wk = wave % WK, wr = wave / WK;
     const int vt = quot(block, A.by_kv), hk = block - vt * A.kv_heads, nk = (int)A.nk;
@@ -1275,8 +1275,10 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
     // at 128 features: one wave's registers fill a SIMD.
     if (A.nq * A.G + A.nk < (int64_t)128 * A.n_seq) return launch_bwd<T, D, 1, 1, 1>(A, s);
     if constexpr (sizeof(T) == 4 && D == 128) return launch_bwd<T, D, 4, 1, 2>(A, s);
-    else if ((A.nk / 128 + A.n_seq + 2) * A.kv_heads >= 4 * 256 && D * sizeof(T) < 256) return launch_bwd<T, D, 4, 1, 2>(A, s);
-    else return launch_bwd<T, D, 4, 2, 2>(A, s);
+    else if ((A.nk / 128 + A.n_seq + 2) * A.kv_heads >= 4 * 256 && D * sizeof(T) < 256)
+        return launch_bwd<T, D, 4, 1, 2>(A, s);
+    else
+        return launch_bwd<T, D, 4, 2, 2>(A, s);
 }
 
 // Splits of the key axis for a cache: enough one-wave blocks for 16 to a CU, and at least 64 keys of the capacity to
@@ -1333,7 +1335,8 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
                   TAGAN_ERR_ARG, "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
-    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: %lld tokens of %d heads",
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
+                  "packed_attn_fwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0) return TAGAN_OK;
     TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_fwd: null offsets");
@@ -1379,7 +1382,8 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
                   TAGAN_ERR_ARG, "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
-    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: %lld tokens of %d heads",
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
+                  "packed_attn_bwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0 && nk == 0) return TAGAN_OK;
     TAGAN_REQUIRE(offsets_q && offsets_k, TAGAN_ERR_ARG, "packed_attn_bwd: null offsets");

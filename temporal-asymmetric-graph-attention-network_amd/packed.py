@@ -41,9 +41,12 @@ def _shapes(*tensors) -> str:
 
 
 def _on_device(first: torch.Tensor, *rest) -> None:
-    require_hip(first, *rest)
+    index = first.get_device()
+    if index < 0:
+        require_hip(first)
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            require_hip(t)
             _refuse("tensors on %s and %s", first.device, t.device)
 
 
