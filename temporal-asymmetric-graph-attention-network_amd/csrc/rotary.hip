@@ -8,8 +8,9 @@
 // block of tokens evaluates its tokens x rot/2 angles once into LDS and reuses them over all heads of q and k.
 //
 // Bound: HBM, two moves of every element: 24001 tokens of 32 + 8 heads of 128, bf16, 492 MB: 97 us, 5.1 TB/s (a copy
-// reaches 4.7); a serving step of 48 tokens: 6 us.  A thread keeps one item (16 B of a head: a vector of each half, or a vector
-// of neighbouring pairs) and steps over the heads, so there is no index division in the loop.
+// reaches 4.7); a serving step of 48 tokens: 6 us.  A thread keeps one item (16 B of a head: a vector of each half, or a
+// vector of neighbouring pairs) and steps over the heads of the block's tokens, so there is no index division in the
+// loop (18889 tokens of 9 heads: 29 us; 47 with one token after the other).
 #include "common.cuh"
 
 namespace tagan {
@@ -78,6 +79,7 @@ template <typename S, bool VEC, int TOK>
 __global__ void __launch_bounds__(RB) k_rotary(RotArgs A) {
     constexpr int E = VEC ? 16 / (int)sizeof(S) : 1;   // elements of an item's vector
     __shared__ float2 cs[TOK * (ROT_MAX_DIM / 2)];
+    __shared__ int64_t in_at[3][TOK], out_at[3][TOK];
     const int half = A.rot / 2;
     const int64_t n0 = (int64_t)blockIdx.x * TOK;
     const int ntok = (int)min((int64_t)TOK, A.tokens - n0);
@@ -90,86 +92,98 @@ __global__ void __launch_bounds__(RB) k_rotary(RotArgs A) {
         sincospif((float)u, &s, &c);
         cs[i] = make_float2(c * A.scale, s * A.scale * A.sign);
     }
+    // where each token's heads lie; an output of -1 is not written
+    if (threadIdx.x < 3 * TOK) {
+        const int which = threadIdx.x / TOK, t = threadIdx.x % TOK;
+        if (t < ntok) {
+            const RotTensor& X = A.x[which];
+            const int64_t n = n0 + t, b = n / A.per, ti = n - b * A.per;
+            int64_t row = ti;
+            if (A.pos == nullptr && which > 0) row += A.lens[b];   // a cache row
+            in_at[which][t] = b * X.ib + ti * X.it;
+            out_at[which][t] = A.pos == nullptr && which > 0 && (row < 0 || row >= A.capacity) ? -1 : b * X.ob + row * X.ot;
+        }
+    }
     __syncthreads();
     // items of a head: the turned ones first, then those that are moved
     const int nrot = A.interleaved ? (VEC ? A.rot / E : half) : half / E;
     const int ntail = (A.dim - A.rot) / E, nall = A.dim / E;
-    for (int t = 0; t < ntok; ++t) {
-        const int64_t n = n0 + t, b = n / A.per, ti = n - b * A.per;
-        for (int which = 0; which < 3; ++which) {
-            const RotTensor& X = A.x[which];
-            if (X.heads == 0) continue;
-            int64_t row = ti;
-            if (A.pos == nullptr && which > 0) {       // a cache row
-                row += A.lens[b];
-                if (row < 0 || row >= A.capacity) continue;
-            }
-            const S* in = (const S*)X.in + b * X.ib + ti * X.it;
-            S* out = (S*)X.out + b * X.ob + row * X.ot;
-            const int items = which == 2 ? nall : nrot + ntail;
-            const int step = RB / items;
-            if ((int)threadIdx.x >= step * items) continue;
-            const int item = threadIdx.x % items;
-            int at, second = -1, pair = 0;             // first feature, the other half's, first pair
-            if (which == 2) at = item * E;
-            else if (item >= nrot) at = A.rot + (item - nrot) * E;
-            else if (!A.interleaved) { at = item * E; second = half + at; pair = at; }
-            else if constexpr (VEC) { at = item * E; second = at; pair = at / 2; }
-            else { at = 2 * item; second = at + 1; pair = item; }
-            const float2* w = cs + t * half + pair;
+    for (int which = 0; which < 3; ++which) {
+        const RotTensor& X = A.x[which];
+        if (X.heads == 0) continue;
+        const int items = which == 2 ? nall : nrot + ntail;
+        const int step = RB / items, rows = ntok * X.heads;   // rows: heads of all tokens
+        if ((int)threadIdx.x >= step * items) continue;
+        const int item = threadIdx.x % items;
+        int at, second = -1, pair = 0;             // first feature, the other half's, first pair
+        if (which == 2) at = item * E;
+        else if (item >= nrot) at = A.rot + (item - nrot) * E;
+        else if (!A.interleaved) { at = item * E; second = half + at; pair = at; }
+        else if constexpr (VEC) { at = item * E; second = at; pair = at / 2; }
+        else { at = 2 * item; second = at + 1; pair = item; }
+        const auto token = [&](int r) {
+            int t = 0;
+#pragma unroll
+            for (int i = 1; i < TOK; ++i) t += r >= i * X.heads;
+            return t;
+        };
+        // U rows at a time, all loads before the first store (outputs may be the inputs, so the compiler keeps their
+        // order): 117 -> 97 us for 24001 tokens of 40 heads
+        constexpr int U = VEC ? 4 : 1;
+        for (int r0 = threadIdx.x / items; r0 < rows; r0 += U * step) {
             if constexpr (VEC) {
-                // U heads at a time, all loads before the first store (outputs may be the inputs, so the compiler keeps
-                // their order): 117 -> 97 us for 24001 tokens of 40 heads
-                constexpr int U = 4;
-                for (int h0 = threadIdx.x / items; h0 < X.heads; h0 += U * step) {
-                    uint4 a[U], b[U];
+                uint4 a[U], b[U];
 #pragma unroll
-                    for (int j = 0; j < U; ++j) {
-                        const int h = min(h0 + j * step, X.heads - 1);
-                        a[j] = *(const uint4*)(in + h * X.ih + at);
-                        if (second > at) b[j] = *(const uint4*)(in + h * X.ih + second);
+                for (int j = 0; j < U; ++j) {
+                    const int r = r0 + j * step, t = token(r);
+                    if (r >= rows) continue;
+                    const S* src = (const S*)X.in + in_at[which][t] + (r - t * X.heads) * X.ih;
+                    a[j] = *(const uint4*)(src + at);
+                    if (second > at) b[j] = *(const uint4*)(src + second);
+                }
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int r = r0 + j * step, t = token(r);
+                    if (r >= rows || out_at[which][t] < 0) continue;
+                    S* dst = (S*)X.out + out_at[which][t] + (r - t * X.heads) * X.oh;
+                    if (second < 0) {
+                        *(uint4*)(dst + at) = a[j];
+                        continue;
                     }
+                    const float2* w = cs + t * half + pair;
+                    float x[E], y[E];
+                    unpack<S>(a[j], x);
+                    if (!A.interleaved) {
+                        unpack<S>(b[j], y);
 #pragma unroll
-                    for (int j = 0; j < U; ++j) {
-                        if (h0 + j * step >= X.heads) break;
-                        S* dst = out + (h0 + j * step) * X.oh;
-                        if (second < 0) {
-                            *(uint4*)(dst + at) = a[j];
-                            continue;
+                        for (int e = 0; e < E; ++e) {
+                            const float c = w[e].x, s = w[e].y, xv = x[e], yv = y[e];
+                            x[e] = xv * c - yv * s;
+                            y[e] = xv * s + yv * c;
                         }
-                        float x[E], y[E];
-                        unpack<S>(a[j], x);
-                        if (!A.interleaved) {
-                            unpack<S>(b[j], y);
+                        *(uint4*)(dst + second) = pack<S>(y);
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < E; ++e) {
-                                const float c = w[e].x, s = w[e].y, xv = x[e], yv = y[e];
-                                x[e] = xv * c - yv * s;
-                                y[e] = xv * s + yv * c;
-                            }
-                            *(uint4*)(dst + second) = pack<S>(y);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const float c = w[e / 2].x, s = w[e / 2].y, xv = x[e], yv = x[e + 1];
-                                x[e] = xv * c - yv * s;
-                                x[e + 1] = xv * s + yv * c;
-                            }
+                        for (int e = 0; e < E; e += 2) {
+                            const float c = w[e / 2].x, s = w[e / 2].y, xv = x[e], yv = x[e + 1];
+                            x[e] = xv * c - yv * s;
+                            x[e + 1] = xv * s + yv * c;
                         }
-                        *(uint4*)(dst + at) = pack<S>(x);
                     }
+                    *(uint4*)(dst + at) = pack<S>(x);
                 }
             } else {
-                for (int h = threadIdx.x / items; h < X.heads; h += step) {
-                    const S* src = in + h * X.ih;
-                    S* dst = out + h * X.oh;
-                    if (second < 0) {
-                        dst[at] = src[at];
-                    } else {
-                        const float xv = ld1(src + at), yv = ld1(src + second), c = w->x, s = w->y;
-                        st1(dst + at, xv * c - yv * s);
-                        st1(dst + second, xv * s + yv * c);
-                    }
+                const int t = token(r0), h = r0 - t * X.heads;
+                if (out_at[which][t] < 0) continue;
+                const S* src = (const S*)X.in + in_at[which][t] + h * X.ih;
+                S* dst = (S*)X.out + out_at[which][t] + h * X.oh;
+                if (second < 0) {
+                    dst[at] = src[at];
+                } else {
+                    const float2* w = cs + t * half + pair;
+                    const float xv = ld1(src + at), yv = ld1(src + second), c = w->x, s = w->y;
+                    st1(dst + at, xv * c - yv * s);
+                    st1(dst + second, xv * s + yv * c);
                 }
             }
         }

@@ -177,10 +177,11 @@ class RotaryFn(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         if dq is None and dk is None:
             return (None,) * 7
+        turn = RotaryFn.apply if torch.is_grad_enabled() else _turn
         if dq is None:
-            dk, _ = RotaryFn.apply(dk, None, positions, inv_freq, *ctx.cfg)
+            dk, _ = turn(dk, None, positions, inv_freq, *ctx.cfg)
         else:
-            dq, dk = RotaryFn.apply(dq, dk, positions, inv_freq, *ctx.cfg)
+            dq, dk = turn(dq, dk, positions, inv_freq, *ctx.cfg)
         return dq, dk, None, None, None, None, None
 
 
