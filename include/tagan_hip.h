@@ -636,13 +636,16 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
  * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
- * gradients.  workspace: tagan_packed_attn_bwd_workspace bytes.
+ * gradients.  workspaces: tagan_packed_attn_fwd_workspace (where few queries meet many keys the key axis is split over
+ * workgroups and joined in a second launch; 0 otherwise) and tagan_packed_attn_bwd_workspace bytes, on 16 bytes.
  * ------------------------------------------------------------------------- */
+size_t tagan_packed_attn_fwd_workspace(int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                                       int32_t head_dim);
 int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
-                          float* lse, void* rest, void* stream);
+                          float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream);
 size_t tagan_packed_attn_bwd_workspace(int64_t nq, int32_t heads);
 int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,

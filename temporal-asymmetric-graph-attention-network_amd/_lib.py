@@ -134,7 +134,8 @@ _SIGNATURES = {
     "tagan_rotary_append": (_c.c_int, [_c.c_int, _i64] + [_i32] * 5 + [_p, _i64, _i64, _i64] * 3 +
                             [_p, _p, _f32, _c.c_int] + [_p, _i64, _i64, _i64] * 3 + [_i64, _p]),
     "tagan_packed_attn_fwd": (_c.c_int, [_c.c_int, _i32, _i64, _i64, _i32, _i32, _i32] + [_p, _i64, _i64] * 3 +
-                              [_p, _p, _c.c_int, _f32, _p, _i64, _i64, _p, _p, _p]),
+                              [_p, _p, _c.c_int, _f32, _p, _i64, _i64, _p, _p, _p, _sz, _p]),
+    "tagan_packed_attn_fwd_workspace": (_sz, [_i32, _i64, _i64, _i32, _i32, _i32]),
     "tagan_packed_attn_bwd_workspace": (_sz, [_i64, _i32]),
     "tagan_packed_attn_bwd": (_c.c_int, [_c.c_int, _i32, _i64, _i64, _i32, _i32, _i32] + [_p, _i64, _i64] * 3 +
                               [_p, _p, _c.c_int, _f32, _p, _i64, _i64, _p, _p] + [_p, _i64, _i64] * 4 + [_p, _sz, _p]),

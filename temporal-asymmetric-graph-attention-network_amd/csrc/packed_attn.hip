@@ -311,7 +311,8 @@ struct AttnArgs {
     Div by_g, by_kv, by_splits, by_tiles;   // of the group, the key heads, the splits, a cache's tiles to a sequence
     float c;                          // scale * log2(e)
     float scale;
-    float* part;                      // splits: sums [row of the batch][split][D], then (base, total) of each
+    float* part;                      // splits: sums [token][head][split][D], then (base, total) of each
+    int64_t part_rows;                // tokens times heads
 };
 
 // One sequence and where its rows lie.  Rows outside every sequence belong to two more that see no key (the run before
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
     if (!R.mine) return;
     if constexpr (SPLIT) {
         // unnormalised sums, and behind those of all rows the maxima (in powers of two) and totals; a row's splits together
-        const int64_t at = ((int64_t)sq.index * A.kv_heads + hk) * R.nrows + R.row;
+        const int64_t at = (sq.index * A.nq + sq.q0 + R.token) * A.heads + hk * A.G + R.g;
         float* p = A.part + (at * A.splits + split) * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -648,8 +649,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
             for (int i = 0; i < 16; i += 4)
                 store4(p + 32 * d + 2 * i + 4 * half, o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
         if (half == 0) {
-            const int64_t all = (int64_t)A.n_seq * A.kv_heads * R.nrows * A.splits;
-            ((float2*)(A.part + all * D))[at * A.splits + split] = make_float2(base, l);
+            ((float2*)(A.part + A.part_rows * A.splits * D))[at * A.splits + split] = make_float2(base, l);
         }
     } else {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -700,11 +700,10 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
     constexpr int JW = JT / 64, JG = JT / 8, CH = D / 32;
     __shared__ float w[JT], red[JW], tot[JW];
     __shared__ float4 sums[JW][8];
-    const int rows = (int)A.nq * A.G;
-    const int64_t all = (int64_t)A.n_seq * A.kv_heads * rows, at = blockIdx.x / CH;
+    const int64_t at = blockIdx.x / CH;
     const int ch = blockIdx.x % CH, s = threadIdx.x, wave = s >> 6, lane = s & 63;
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (s < A.splits) ml = ((const float2*)(A.part + all * A.splits * D))[at * A.splits + s];
+    if (s < A.splits) ml = ((const float2*)(A.part + A.part_rows * A.splits * D))[at * A.splits + s];
     const bool some = ml.y != 0.f;             // a split without a visible key has no base
     const float m = lane_max<64>(some ? ml.x : -INFINITY);
     if (lane == 0) red[wave] = m;
@@ -751,12 +750,19 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const int64_t bh = at / rows;
-    const int row = (int)(at - bh * rows), token = quot(row, A.by_g);
-    const int64_t b = bh / A.kv_heads;
-    const int head = (int)(bh - b * A.kv_heads) * A.G + row - token * A.G;
-    T* out = (T*)A.out + b * A.os.b + (int64_t)token * A.os.tok + (int64_t)head * A.os.head;
-    store4(out + feature, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const int64_t token = at / A.heads, head = at - token * A.heads, b = token / A.nq;   // packed: one batch of nq tokens
+    T* out = (T*)A.out + b * A.os.b + (token - b * A.nq) * A.os.tok + head * A.os.head;
+    const float x4[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    store4(out + feature, x4[0], x4[1], x4[2], x4[3]);
+    if (A.lse && s == 0 && ch == 0) A.lse[at] = l == 0.f ? INFINITY : top + __log2f(l);
+    if constexpr (sizeof(T) == 2) {
+        if (A.rest) {
+            float r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = x4[j] - __uint_as_float(f2bf2(x4[j], 0.f) << 16);
+            store4(A.rest + at * A.dim + feature, r[0], r[1], r[2], r[3]);
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -1236,19 +1242,6 @@ int check_tensor(const char* what, const char* name, const void* p, Strides& s, 
 // a launch counts its threads in 32 bits
 bool fits_grid(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads && blocks <= 0x7fffffff; }
 
-template <typename T, int D>
-int run_fwd(const AttnArgs& A, hipStream_t s) {
-    // waves to a block by the rows that a sequence has on average: 32-row blocks where four waves would mostly idle
-    const bool one = A.nq * A.G < (int64_t)64 * A.n_seq;
-    const int rows = one ? 32 : 128;
-    const int64_t blocks = (A.nq * A.G / rows + A.n_seq + 2) * A.kv_heads;
-    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256), TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
-    if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
-    else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
-    TAGAN_CHECK_LAUNCH("packed_attn_fwd");
-    return TAGAN_OK;
-}
-
 template <typename T, int D, int WK, int WR, int STAGES>
 int launch_bwd(AttnArgs A, hipStream_t s) {
     const int64_t keys = A.nk > 0 ? (A.nk / (32 * WK) + A.n_seq + 2) * A.kv_heads : 0;
@@ -1281,39 +1274,75 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
         return launch_bwd<T, D, 4, 2, 2>(A, s);
 }
 
-// Splits of the key axis for a cache: enough one-wave blocks for 16 to a CU, and at least 64 keys of the capacity to
-// each (the lengths themselves are on the device; a split divides the length it finds there)
-int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity, bool one) {
-    const int64_t blocks = batch * kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128));
+// Splits of the key axis where rows are few: enough one-wave blocks for 16 to a CU, and at least `least` keys of the longest
+// axis to each (the lengths themselves are on the device; a split divides the length it finds there).
+int key_splits(int64_t blocks, bool one, int64_t keys, int64_t least) {
     const int64_t want = ((one ? 4096 : 1024) + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = (capacity + 63) / 64;
+    const int64_t most = (keys + least - 1) / least;
     const int64_t n = want < most ? want : most;
     return (int)(n < 1 ? 1 : n > MAX_SPLITS ? MAX_SPLITS : n);
 }
-bool cache_one(int64_t rows) { return rows < 64; }
+bool few_rows(int64_t rows) { return rows < 64; }   // of a sequence: one-wave blocks, four waves would mostly idle
+int64_t cache_blocks(int64_t batch, int64_t rows, int64_t kv_heads) {
+    return batch * kv_heads * (few_rows(rows) ? (rows + 31) / 32 : (rows + 127) / 128);
+}
+int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity) {
+    return key_splits(cache_blocks(batch, rows, kv_heads), few_rows(rows), capacity, 64);
+}
+// Packed sequences: blocks by the rows of an average sequence, splits by its keys, 256 to each and 32 MB of partial sums at
+// most.  16 x 8 tokens on 8192 keys, 8 heads over 2, 128 bf16 features: 330 us unsplit, 41 split.
+int64_t packed_blocks(int64_t n_seq, int64_t nq, int64_t G, int64_t kv_heads) {
+    return (nq * G / (nq * G < 64 * n_seq ? 32 : 128) + n_seq + 2) * kv_heads;
+}
+int packed_splits(int64_t n_seq, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int D) {
+    if (n_seq < 1 || nq < 1 || nk < 512 * n_seq) return 1;
+    const int64_t G = heads / kv_heads, row = heads * nq * (D + 2) * 4, budget = (32ll << 20) / row;
+    const int n = key_splits(packed_blocks(n_seq, nq, G, kv_heads), nq * G < 64 * n_seq, nk / n_seq, 256);
+    return n < budget ? n : budget < 2 ? 1 : (int)budget;
+}
 
 template <typename T, int D>
-int run_cached(const AttnArgs& A, hipStream_t s) {
-    const int64_t rows = A.nq * A.G;
-    const bool one = cache_one(rows);
-    const int64_t blocks = (int64_t)A.n_seq * A.kv_heads * ((rows + (one ? 31 : 127)) / (one ? 32 : 128)) * A.splits;
-    const int64_t joins = (int64_t)A.n_seq * A.kv_heads * rows * (D / 32);
-    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256) && fits_grid(joins, 512), TAGAN_ERR_UNSUPPORTED,
-                  "cached_attn: too many rows");
-    if (A.splits == 1) {
-        if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
-        else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
-        TAGAN_CHECK_LAUNCH("cached_attn");
-        return TAGAN_OK;
-    }
+int launch_splits(const AttnArgs& A, int64_t blocks, bool one, const char* what, hipStream_t s) {
+    const int64_t joins = A.part_rows * (D / 32);
+    TAGAN_REQUIRE(fits_grid(blocks * A.splits, one ? 64 : 256) && fits_grid(joins, 512), TAGAN_ERR_UNSUPPORTED,
+                  "%s: too many rows", what);
+    const unsigned grid = (unsigned)(blocks * A.splits);
     // 32 keys and values of 128 fp32 features are 32 KB: twice that would leave two waves to a CU
-    if (one) k_attn_fwd<T, D, 1, true, sizeof(T) == 4 && D == 128 ? 1 : 2><<<(unsigned)blocks, 64, 0, s>>>(A);
-    else k_attn_fwd<T, D, 4, true, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
-    TAGAN_CHECK_LAUNCH("cached_attn");
+    if (one) k_attn_fwd<T, D, 1, true, sizeof(T) == 4 && D == 128 ? 1 : 2><<<grid, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, true, 2><<<grid, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH(what);
     static_assert(MAX_SPLITS <= 512, "a thread to a split");
     if (A.splits <= 64) k_attn_join<T, D, 64><<<(unsigned)joins, 64, 0, s>>>(A);
     else k_attn_join<T, D, 512><<<(unsigned)joins, 512, 0, s>>>(A);
-    TAGAN_CHECK_LAUNCH("cached_attn (join)");
+    TAGAN_CHECK_LAUNCH(what);
+    return TAGAN_OK;
+}
+
+template <typename T, int D>
+int run_fwd(const AttnArgs& A, hipStream_t s) {
+    const bool one = A.nq * A.G < (int64_t)64 * A.n_seq;
+    const int64_t blocks = packed_blocks(A.n_seq, A.nq, A.G, A.kv_heads);
+    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256), TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
+    if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("packed_attn_fwd");
+    return TAGAN_OK;
+}
+template <typename T, int D>
+int run_fwd_splits(const AttnArgs& A, hipStream_t s) {
+    return launch_splits<T, D>(A, packed_blocks(A.n_seq, A.nq, A.G, A.kv_heads), A.nq * A.G < (int64_t)64 * A.n_seq,
+                               "packed_attn_fwd", s);
+}
+
+template <typename T, int D>
+int run_cached(const AttnArgs& A, hipStream_t s) {
+    const int64_t rows = A.nq * A.G, blocks = cache_blocks(A.n_seq, rows, A.kv_heads);
+    const bool one = few_rows(rows);
+    if (A.splits > 1) return launch_splits<T, D>(A, blocks, one, "cached_attn", s);
+    TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256), TAGAN_ERR_UNSUPPORTED, "cached_attn: too many rows");
+    if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
+    else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
+    TAGAN_CHECK_LAUNCH("cached_attn");
     return TAGAN_OK;
 }
 
@@ -1326,11 +1355,18 @@ using namespace tagan;
 
 extern "C" {
 
+size_t tagan_packed_attn_fwd_workspace(int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
+                                       int32_t head_dim) {
+    if (kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
+    const int n = packed_splits(n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim));
+    return n == 1 ? 0 : (size_t)n * (size_t)nq * (size_t)heads * (size_t)(padded_dim(head_dim) + 2) * 4;
+}
+
 int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
                           int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* offsets_q,
                           const int32_t* offsets_k, int causal, float scale, void* out, int64_t o_tok, int64_t o_head,
-                          float* lse, void* rest, void* stream) {
+                          float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("packed_attn_fwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
     TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
@@ -1358,11 +1394,22 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     A.offs_q = offsets_q; A.offs_k = offsets_k;
     A.nq = nq; A.nk = nk; A.n_seq = n_seq;
     A.heads = heads; A.kv_heads = kv_heads; A.G = heads / kv_heads; A.dim = head_dim;
-    A.causal = causal != 0; A.splits = 1;
+    A.causal = causal != 0;
     A.by_g = div_by(A.G);
     A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     hipStream_t s = as_stream(stream);
+    const size_t need = tagan_packed_attn_fwd_workspace(n_seq, nq, nk, heads, kv_heads, head_dim);
+    TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)),
+                  TAGAN_ERR_WORKSPACE, "packed_attn_fwd: workspace of %zu bytes, %zu are needed on 16", workspace_bytes, need);
+    A.splits = need ? packed_splits(n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim)) : 1;
+    if (A.splits > 1) {
+        A.by_splits = div_by(A.splits);
+        A.part = (float*)workspace;
+        A.part_rows = nq * heads;
+        return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_fwd_splits)(A, s)
+                                  : TAGAN_BY_DIM(uint16_t, head_dim, run_fwd_splits)(A, s);
+    }
     return dtype == TAGAN_F32 ? TAGAN_BY_DIM16(float, head_dim, run_fwd)(A, s)
                               : TAGAN_BY_DIM16(uint16_t, head_dim, run_fwd)(A, s);
 }
@@ -1431,7 +1478,7 @@ size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capac
                                    int32_t head_dim) {
     if (batch <= 0 || new_len <= 0 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
     const int64_t rows = (int64_t)new_len * (heads / kv_heads);
-    const int n = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
+    const int n = cache_splits(batch, rows, kv_heads, capacity);
     return n == 1 ? 0 : (size_t)n * (size_t)batch * (size_t)(kv_heads * rows) * (size_t)(padded_dim(head_dim) + 2) * 4;
 }
 
@@ -1470,13 +1517,14 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
     A.by_kv = div_by(kv_heads);
     A.scale = scale; A.c = scale * LOG2E;
     const int64_t rows = (int64_t)new_len * A.G;
-    A.splits = cache_splits(batch, rows, kv_heads, capacity, cache_one(rows));
+    A.splits = cache_splits(batch, rows, kv_heads, capacity);
     A.by_splits = div_by(A.splits);
-    A.by_tiles = div_by((rows + (cache_one(rows) ? 31 : 127)) / (cache_one(rows) ? 32 : 128));
+    A.by_tiles = div_by(few_rows(rows) ? (rows + 31) / 32 : (rows + 127) / 128);
     A.part = (float*)workspace;
+    A.part_rows = batch * new_len * heads;
     const size_t need = tagan_cached_attn_workspace(batch, new_len, capacity, heads, kv_heads, head_dim);
-    TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), TAGAN_ERR_WORKSPACE,
-                  "cached_attn: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+    TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)),
+                  TAGAN_ERR_WORKSPACE, "cached_attn: workspace of %zu bytes, %zu are needed on 16", workspace_bytes, need);
     hipStream_t s = as_stream(stream);
     return dtype == TAGAN_F32 ? TAGAN_BY_DIM(float, head_dim, run_cached)(A, s)
                               : TAGAN_BY_DIM(uint16_t, head_dim, run_cached)(A, s);

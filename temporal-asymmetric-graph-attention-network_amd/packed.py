@@ -268,10 +268,13 @@ class PackedAttnFn(torch.autograd.Function):
         lse = torch.empty((n, heads), dtype=torch.float32, device=q.device) if needs else None
         rest = torch.empty_like(out) if needs and q.dtype is torch.bfloat16 else None
         if n:
+            size = lib().tagan_packed_attn_fwd_workspace(offsets.shape[0] - 1, n, nk, heads, hk, d)
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
             _run("tagan_packed_attn_fwd", q, dtype_code(q), offsets.shape[0] - 1, n, nk, heads, hk, d, q.data_ptr(),
                  *q.stride()[:2], k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2], offsets.data_ptr(),
                  offsets_k.data_ptr(), causal, scale, out.data_ptr(), heads * d, d,
-                 lse.data_ptr() if needs else None, None if rest is None else rest.data_ptr())
+                 lse.data_ptr() if needs else None, None if rest is None else rest.data_ptr(),
+                 ws.data_ptr() if size else None, size)
         if needs:
             ctx.save_for_backward(q, k, v, out, lse, rest, offsets, offsets_k)
             ctx.cfg = (causal, scale)
@@ -318,8 +321,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
 
     Queries that see no key (an empty history, or Lq > Lk with ``causal``) and tokens outside every history (before
     the first offset, behind the last) give zeros and get zero gradients; offsets beyond the token count are taken as
-    the token count.  What a query does not see, infinities and NaN included, does not reach its output.
-    A few queries against a long history are ``cached_attention``'s: it splits the key axis, this does not.  Gradients
+    the token count.  What a query does not see, infinities and NaN included, does not reach its output.  Gradients
     flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.  There is
     no second derivative (``create_graph`` raises).
     """

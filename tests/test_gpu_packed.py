@@ -164,6 +164,18 @@ def test_more_or_fewer_keys_than_queries(dtype, causal, lens, klens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_few_queries_on_many_keys(dtype, causal, d):
+    """The key axis is split over workgroups and joined: one-wave and four-wave blocks, empty sequences, empty tails."""
+    assert packed.lib().tagan_packed_attn_fwd_workspace(4, 12, 6301, 4, 2, d) > 0
+    assert packed.lib().tagan_packed_attn_fwd_workspace(2, 150, 5000, 4, 2, d) > 0
+    _attend([1, 8, 0, 3], [3000, 700, 600, 2001], 4, 2, d, dtype, causal, first=0, tail=0)
+    _attend([130, 20], [4000, 1000], 4, 2, d, dtype, causal)
+    _attend([5, 1], [1500, 0], 2, 2, d, dtype, causal, first=9, tail=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_wide_groups(dtype):
     _attend([20, 3], [45, 3], 100, 1, 16, dtype)
     _attend([2], [5], 512, 1, 8, dtype)

@@ -136,16 +136,16 @@ def test_append_refuses_shared_cache_rows():
 A = 0x10000   # a pointer that is never followed
 
 
-def _fwd(L, dtype=0, n_seq=1, nq=4, nk=4, heads=4, kv=2, d=16, q=A, tok=64, head=16, offs=A, scale=0.25):
+def _fwd(L, dtype=0, n_seq=1, nq=4, nk=4, heads=4, kv=2, d=16, q=A, tok=64, head=16, offs=A, scale=0.25, ws=None, size=0):
     return L.tagan_packed_attn_fwd(dtype, n_seq, nq, nk, heads, kv, d, q, tok, head, A, 32, 16, A, 32, 16, offs, offs,
-                                   1, scale, A, 64, 16, None, None, None)
+                                   1, scale, A, 64, 16, None, None, ws, size, None)
 
 
 @pytest.mark.parametrize("kw, status", [
     (dict(dtype=2), -2), (dict(d=12), -2), (dict(d=136), -2), (dict(heads=5), -1), (dict(kv=0), -1),
     (dict(heads=1026, kv=2), -1), (dict(scale=0.0), -1), (dict(nq=-1), -1), (dict(nk=1 << 31), -1), (dict(n_seq=-1), -1),
     (dict(q=None), -1), (dict(q=A + 4), -1), (dict(tok=66), -1), (dict(tok=8), -1), (dict(tok=1 << 23), -1),
-    (dict(offs=None), -1), (dict(nq=0, q=None), 0),
+    (dict(offs=None), -1), (dict(nq=0, q=None), 0), (dict(nk=4000), -4), (dict(nk=4000, ws=A + 8, size=1 << 30), -4),
 ])
 def test_packed_fwd_entry(kw, status):
     assert _fwd(_lib.lib(), **kw) == status
