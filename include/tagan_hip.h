@@ -634,10 +634,12 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * bytes, feature stride 1, token strides of head_dim to 2^21, tokens times heads / kv_heads below 2^31.
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
  * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
- * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values (infinities and NaN too) of keys that a row does not see never reach that row's output.
+ * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values
+ * (infinities and NaN too) of keys that a row does not see never reach that row's output.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
  * gradients.  workspaces: tagan_packed_attn_fwd_workspace (where few queries meet many keys the key axis is split over
- * workgroups and joined in a second launch; 0 otherwise) and tagan_packed_attn_bwd_workspace bytes, on 16 bytes.
+ * workgroups and joined in a second launch; 0 otherwise; enough for either type) and tagan_packed_attn_bwd_workspace
+ * bytes, on 16 bytes.
  * ------------------------------------------------------------------------- */
 size_t tagan_packed_attn_fwd_workspace(int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                                        int32_t head_dim);

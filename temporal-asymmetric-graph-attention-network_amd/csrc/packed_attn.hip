@@ -1289,15 +1289,22 @@ int64_t cache_blocks(int64_t batch, int64_t rows, int64_t kv_heads) {
 int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity) {
     return key_splits(cache_blocks(batch, rows, kv_heads), few_rows(rows), capacity, 64);
 }
-// Packed sequences: blocks by the rows of an average sequence, splits by its keys, 256 to each and 32 MB of partial sums at
-// most.  16 x 8 tokens on 8192 keys, 8 heads over 2, 128 bf16 features: 330 us unsplit, 41 split.
+// Packed sequences: blocks by the rows of an average sequence, splits by its keys, at least 256 to each.  A block takes
+// about `key` ns to a key (measured); where that comes to 20 us the axis is split, into as many as write their sums in a
+// quarter of that time (written and read at 3 TB/s), 64 MB at most.  Unsplit and split, 128 features: 16 x 8 tokens on 8192
+// keys, bf16, 8 heads over 2: 330 and 41 us; one causal history of 4096, a head: bf16 102 and 29 us, fp32 538 and 70 us;
+// two of 1024, 8 heads, bf16, stay unsplit: 33 and 46 us.
 int64_t packed_blocks(int64_t n_seq, int64_t nq, int64_t G, int64_t kv_heads) {
     return (nq * G / (nq * G < 64 * n_seq ? 32 : 128) + n_seq + 2) * kv_heads;
 }
-int packed_splits(int64_t n_seq, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int D) {
-    if (n_seq < 1 || nq < 1 || nk < 512 * n_seq) return 1;
-    const int64_t G = heads / kv_heads, row = heads * nq * (D + 2) * 4, budget = (32ll << 20) / row;
-    const int n = key_splits(packed_blocks(n_seq, nq, G, kv_heads), nq * G < 64 * n_seq, nk / n_seq, 256);
+int packed_splits(int dtype, int64_t n_seq, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int D) {
+    if (n_seq < 1 || nq < 1 || nk < 1) return 1;
+    const int64_t G = heads / kv_heads, keys = nk / n_seq, row = heads * nq * (D + 2) * 4;
+    const bool one = nq * G < 64 * n_seq;
+    const int64_t key = (dtype == TAGAN_F32 ? 10 + D : 6 + D / 7) * (one ? 3 : 2) / 2, ns = keys * key;
+    if (ns < 20000) return 1;
+    const int64_t bytes = ns * 375, most = 64ll << 20, budget = (bytes < most ? bytes : most) / row;
+    const int n = key_splits(packed_blocks(n_seq, nq, G, kv_heads), one, keys, 256);
     return n < budget ? n : budget < 2 ? 1 : (int)budget;
 }
 
@@ -1358,7 +1365,7 @@ extern "C" {
 size_t tagan_packed_attn_fwd_workspace(int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                                        int32_t head_dim) {
     if (kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
-    const int n = packed_splits(n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim));
+    const int n = packed_splits(TAGAN_F32, n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim));   // bf16 splits no more
     return n == 1 ? 0 : (size_t)n * (size_t)nq * (size_t)heads * (size_t)(padded_dim(head_dim) + 2) * 4;
 }
 
@@ -1402,7 +1409,7 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
     const size_t need = tagan_packed_attn_fwd_workspace(n_seq, nq, nk, heads, kv_heads, head_dim);
     TAGAN_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)),
                   TAGAN_ERR_WORKSPACE, "packed_attn_fwd: workspace of %zu bytes, %zu are needed on 16", workspace_bytes, need);
-    A.splits = need ? packed_splits(n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim)) : 1;
+    A.splits = need ? packed_splits(dtype, n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim)) : 1;
     if (A.splits > 1) {
         A.by_splits = div_by(A.splits);
         A.part = (float*)workspace;

@@ -176,6 +176,14 @@ def test_few_queries_on_many_keys(dtype, causal, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [([2, 0, 5, 1], [9000, 300, 4100, 1]), ([300], [2300]), ([1100, 1], [1100, 2500])])
+def test_long_keys_for_few_blocks(dtype, lens):
+    """Axes long enough to be split in both types: one-wave blocks, one history of many rows, uneven ones."""
+    assert packed.lib().tagan_packed_attn_fwd_workspace(len(lens[0]), sum(lens[0]), sum(lens[1]), 2, 1, 64) > 0
+    _attend(*lens, 2, 1, 64, dtype, True, first=0, tail=0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_wide_groups(dtype):
     _attend([20, 3], [45, 3], 100, 1, 16, dtype)
     _attend([2], [5], 512, 1, 8, dtype)
