@@ -320,6 +320,7 @@ struct AttnArgs {
 struct Seq {
     int q0, k0;        // first token, first key
     int lq, lk, index;
+    int past;          // keys before the first query's own; of a cache by its length, fit or not
     int tile;          // tile of this sequence
 };
 
@@ -413,7 +414,9 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
         s.tile = vt - s.index * (int)A.by_tiles.d;
         s.lq = (int)A.nq;
         s.q0 = s.k0 = 0;
-        s.lk = max(0, min((int)A.nk, A.lens[s.index]));
+        const int len = max(0, A.lens[s.index]);
+        s.lk = min((int)A.nk, len);
+        s.past = len - s.lq;
         return true;
     }
     const Found f = find_seq(A.offs_q, A.n_seq, (int)A.nq, A.G, ROWS, vt);
@@ -433,12 +436,13 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
             s.lk = max(0, edge(A.offs_k, A.n_seq, (int)A.nk, f.i + 1) - s.k0);
         }
     }
+    s.past = s.lk - s.lq;
     return true;
 }
 
 // The rows of a wave and what they see.  Counts of rows (tokens times the group) stay below 2^31.
 struct Rows {
-    int nrows, r0, row, token, g, past;
+    int nrows, r0, row, token, g;
     bool mine;
     int see;                           // keys of this lane's row
     int most, least;                   // keys that some row of the block sees, and that all of its rows see
@@ -454,9 +458,8 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs& A, const Seq& sq) {
     R.mine = R.row < R.nrows;
     R.token = quot(R.row, A.by_g);
     R.g = R.row - R.token * A.G;
-    R.past = sq.lk - sq.lq;            // keys before the first query's own
-    const auto keys = [&](int row) { return A.causal ? min(sq.lk, max(0, quot(row, A.by_g) + R.past + 1)) : sq.lk; };
-    R.see = !R.mine ? 0 : (A.causal ? min(sq.lk, max(0, R.token + R.past + 1)) : sq.lk);
+    const auto keys = [&](int row) { return A.causal ? min(sq.lk, max(0, quot(row, A.by_g) + sq.past + 1)) : sq.lk; };
+    R.see = !R.mine ? 0 : (A.causal ? min(sq.lk, max(0, R.token + sq.past + 1)) : sq.lk);
     R.most = keys(min(R.r0 + ROWS, R.nrows) - 1);
     R.least = keys(R.r0);
     const int w0 = R.r0 + wave * 32;

@@ -350,9 +350,10 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: Optional[float] = None) -> torch.Tensor:
     """New tokens against the cache: q [B, L, heads, d], caches [B, capacity, kv_heads, d] -> [B, L, heads, d].
 
-    ``lens`` [B] int32 counts the cached rows of each history, the L new ones included: query i sees rows
-    j < lens[b] - L + 1 + i, and zeros come back where that is none.  Rows from ``lens[b]`` on are not used, whatever
-    they hold.  The caches are read in place: unit feature stride, other strides and the start on 16 bytes, token strides
+    ``lens`` [B] int32 counts the tokens of each history, the L new ones included: query i sees the rows
+    j < lens[b] - L + 1 + i of the cache, and zeros come back where that is none.  A length past the capacity leaves
+    that window where it is (the rows that ``rotary_append`` had no room for are missing from it).  Rows from ``lens[b]``
+    on are not used, whatever they hold.  The caches are read in place: unit feature stride, other strides and the start on 16 bytes, token strides
     up to 2^21 elements (RuntimeError otherwise).  No autograd."""
     _storage(q, k_cache, v_cache)
     _cache(k_cache, "k_cache")

@@ -1,0 +1,113 @@
+"""Edges of the packed operators: bounds that a wrong result cannot pass, caches past their capacity, infinities, limits.
+
+Inputs are made on the CPU, so that the checks of the bounds themselves run without a device: a bound has to refuse a
+planted mistake (in the 64-bit reference).  Bounds, with W = 2^-24 and u half a step of the storage type:
+  scores   |ds| <= (d + 4) W scale |q||k|; the exponent's argument (at most 8 powers of two above the maximum's) and
+           exp2 add (|s - m| + 16) W: a relative error e of each unnormalised weight, 2 e of each normalised one
+  out      the sum over S keys adds (S + 8) W, the join of at most 512 splits 2 (512 + 8) W (its weights and its sum):
+           |do| <= (u' + 2 e + (S + 8 + 2 * 520) W) P|V| + u |o|, u' = u for bf16 (each probability is rounded), else 0
+"""
+import math
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from tagan_amd import _lib, packed
+
+DEV = "cuda"
+W = 2.0 ** -24
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+DTYPES = [torch.float32, torch.bfloat16]
+I32 = torch.int32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(gen, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=gen).to(dtype)
+
+
+def _rows(q, k, v, see, scale, dtype):
+    """softmax(scale q kᵀ) v of the keys that `see` [R, S] shows, in 64 bits: out [R, d], its bound and the weights."""
+    q, k, v = q.double(), k.double(), v.double()
+    u, u1, d, S = UNIT[dtype], UNIT[dtype] if dtype == torch.bfloat16 else 0.0, q.shape[1], k.shape[0]
+    s = ((q @ k.T) * scale).masked_fill(~see, -math.inf)
+    m = s.amax(1, keepdim=True) if S else torch.zeros(q.shape[0], 1, dtype=torch.float64)
+    m = torch.where(torch.isfinite(m), m, 0.0)
+    P = torch.exp(s - m)
+    total = P.sum(1, keepdim=True)
+    P = P / torch.where(total > 0, total, 1.0)
+    sab = (q.abs() @ k.abs().T) * scale
+    e = ((d + 4) * W * sab + ((s - m).abs() + 16) * W).masked_fill(~see, 0.0)
+    e = e.amax(1, keepdim=True) if S else torch.zeros_like(m)
+    o = P @ v
+    return o, (u1 + 2 * e + (S + 8 + 2 * 520) * W) * (P @ v.abs()) * (1 + u) + u * o.abs(), P
+
+
+def _cached_want(q, kc, vc, lens, scale=None):
+    """cached_attention and its bound on the CPU: query i sees rows j < lens - L + 1 + i of the cache."""
+    B, L, hq, d = q.shape
+    cap, hk = kc.shape[1:3]
+    G, scale = hq // hk, d ** -0.5 if scale is None else scale
+    out, tol = torch.zeros(B, L, hq, d, dtype=torch.float64), torch.zeros(B, L, hq, d, dtype=torch.float64)
+    for b, n in enumerate(lens):
+        S = max(0, min(n, cap))
+        end = torch.tensor([n - L + 1 + i for i in range(L) for _ in range(G)])
+        see = torch.arange(S)[None] < end[:, None]
+        for h in range(hk):
+            sl = slice(h * G, (h + 1) * G)
+            o, t, _ = _rows(q[b, :, sl].reshape(L * G, d), kc[b, :S, h], vc[b, :S, h], see, scale, q.dtype)
+            out[b, :, sl], tol[b, :, sl] = o.view(L, G, d), t.view(L, G, d)
+    return out, tol
+
+
+def _within(got, want, tol, what):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape and bool(torch.isfinite(got).all()), what
+    over = (got - want).abs() - tol
+    assert not bool((over > 0).any()), "%s: %d of %d beyond their bound, worst by %.3g" % (
+        what, int((over > 0).sum()), over.numel(), float(over.max()))
+
+
+def _dev(*tensors):
+    return [t.to(DEV) for t in tensors]
+
+
+# ----------------------------------------------------------------------------- a cache whose lengths pass its capacity
+PAST = [(50, 5, [52, 50, 54, 55, 56, 2 ** 31 - 1, 45, 3, -2 ** 31], 8, 2, 64), (3000, 3, [3002, 3001, 3000, 3500], 4, 1, 128),
+        (20, 40, [25, 59, 60, 7], 4, 2, 16), (0, 2, [0, 2, 9], 2, 1, 32)]
+
+
+def _past(cap, L, lens, hq, hk, d, dtype):
+    gen = _gen(21)
+    q = _randn(gen, len(lens), L, hq, d, dtype=dtype)
+    return q, *(_randn(gen, len(lens), cap, hk, d, dtype=dtype) for _ in range(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cap, L, lens, hq, hk, d", PAST)
+def test_lengths_past_the_capacity_keep_the_window(dtype, cap, L, lens, hq, hk, d):
+    """The rows that did not fit are missing, but each query still sees what lies before it."""
+    q, kc, vc = _past(cap, L, lens, hq, hk, d, dtype)
+    got = packed.cached_attention(*_dev(q, kc, vc, torch.tensor(lens, dtype=I32)))
+    _within(got, *_cached_want(q, kc, vc, lens), "capacity %d, new %d" % (cap, L))
+
+
+@pytest.mark.gpu
+def test_append_past_the_capacity_then_attend():
+    """Three of five new tokens fit: each of them sees its own key, and so do those that follow."""
+    gen, cap, L, hq, hk, d = _gen(22), 50, 5, 4, 2, 32
+    q, k, v = (_randn(gen, 1, L, h, d) for h in (hq, hk, hk))
+    kc, vc = _dev(_randn(gen, 1, cap, hk, d), _randn(gen, 1, cap, hk, d))
+    freq, _ = packed.rotary_frequencies(d, device=DEV)
+    lens = torch.tensor([47], dtype=I32, device=DEV)
+    qn = packed.rotary_append(*_dev(q, k, v), kc, vc, lens, freq)
+    lens += L
+    got = packed.cached_attention(qn, kc, vc, lens)
+    assert torch.equal(vc[0, 47:].cpu(), v[0, :3])
+    _within(got, *_cached_want(qn.cpu(), kc.cpu(), vc.cpu(), [52]), "after the last row")
