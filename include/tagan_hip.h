@@ -635,7 +635,8 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
  * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
  * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values
- * (infinities and NaN too) of keys that a row does not see never reach that row's output.
+ * (infinities and NaN too) of keys that a row does not see never reach that row's output; an infinite or NaN value that
+ * it sees makes that feature of its output infinite or NaN, however small the weight.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
  * gradients.  workspaces: tagan_packed_attn_fwd_workspace (where few queries meet many keys the key axis is split over
  * workgroups and joined in a second launch; 0 otherwise; enough for either type) and tagan_packed_attn_bwd_workspace

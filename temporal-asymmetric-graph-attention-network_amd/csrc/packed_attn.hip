@@ -232,7 +232,8 @@ struct Tile {
 
 // Infinities and NaN among the values of a tile of which some row sees only a part: 0 * inf in the product would carry
 // them into rows that do not see them.  Such a tile is multiplied with zeros in their place, and after the last tile
-// each row adds those that it does see (any weight times an infinity is that infinity).
+// each row adds those that it does see (any weight times an infinity is that infinity).  Elsewhere a weight that is zero
+// in fp32 makes NaN of it: either way a row that sees such a value is not finite there.
 __device__ __forceinline__ bool wild(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 template <typename T>
 __device__ __forceinline__ bool tame(uint32_t& w) {
@@ -727,14 +728,14 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int i = g; i < A.splits; i += JG) {
+        // a split that the row does not see has zeros here; one whose weight is zero may hold an infinity that the row
+        // does see, and 0 * inf tells so
         const float4 v = *(const float4*)(p + (int64_t)i * D);
         const float wi = w[i];
-        if (wi != 0.f) {                       // NaN weights too
-            o.x = fmaf(v.x, wi, o.x);
-            o.y = fmaf(v.y, wi, o.y);
-            o.z = fmaf(v.z, wi, o.z);
-            o.w = fmaf(v.w, wi, o.w);
-        }
+        o.x = fmaf(v.x, wi, o.x);
+        o.y = fmaf(v.y, wi, o.y);
+        o.z = fmaf(v.z, wi, o.z);
+        o.w = fmaf(v.w, wi, o.w);
     }
 #pragma unroll
     for (int d = 8; d < 64; d <<= 1) {

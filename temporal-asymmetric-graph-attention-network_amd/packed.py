@@ -321,7 +321,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
 
     Queries that see no key (an empty history, or Lq > Lk with ``causal``) and tokens outside every history (before
     the first offset, behind the last) give zeros and get zero gradients; offsets beyond the token count are taken as
-    the token count.  What a query does not see, infinities and NaN included, does not reach its output.  Gradients
+    the token count.  What a query does not see, infinities and NaN included, does not reach its output; an infinity or
+    NaN in a value that it sees makes that feature of its output infinite or NaN, however small the weight.  Gradients
     flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.  There is
     no second derivative (``create_graph`` raises).
     """

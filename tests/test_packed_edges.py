@@ -111,3 +111,39 @@ def test_append_past_the_capacity_then_attend():
     got = packed.cached_attention(qn, kc, vc, lens)
     assert torch.equal(vc[0, 47:].cpu(), v[0, :3])
     _within(got, *_cached_want(qn.cpu(), kc.cpu(), vc.cpu(), [52]), "after the last row")
+
+
+# ----------------------------------------------------------------------------- infinities that a row sees
+def _hidden_weight(n, hk, d, at, bad, gen):
+    """Keys 0 to 511 weigh nothing in fp32 (their scores lie 120 below the others'); one of their values is `bad`."""
+    k, v = _randn(gen, n, hk, d), _randn(gen, n, hk, d)
+    k[:, :, 0] = 0
+    k[:512, :, 0] = -120 * d ** 0.5
+    v[at, :, 3] = bad
+    return k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("d", [16, 128])
+def test_what_a_row_sees_reaches_it_whatever_its_weight(dtype, bad, d):
+    """In one pass over the keys and in splits of them, packed and cached: no finite result hides such a value."""
+    gen, n, at = _gen(23), 6000, 70
+    k, v = (t.to(dtype) for t in _hidden_weight(n, 1, d, at, bad, gen))
+    q = torch.zeros(n, 2, d, dtype=dtype)
+    q[:, :, 0] = 1
+    k, v, q = _dev(k, v, q)
+    offs = [torch.tensor([0, m], dtype=I32, device=DEV) for m in (1, 3, n)]
+
+    def seen(out, rows):
+        assert not bool(torch.isfinite(out[rows, :, 3]).any())
+        assert bool(torch.isfinite(out[rows][..., [0, 1, 2, *range(4, d)]]).all())
+    assert packed.lib().tagan_packed_attn_fwd_workspace(1, 1, n, 2, 1, d) > 0
+    seen(packed.attention(q[:1], k, v, offs[0], offs[2]), slice(0, 1))
+    seen(packed.attention(q[:3], k, v, offs[1], offs[2], causal=False), slice(0, 3))
+    out = packed.attention(q[:900], k[:900], v[:900], torch.tensor([0, 900], dtype=I32, device=DEV))
+    assert bool(torch.isfinite(out[:at]).all())
+    seen(out, slice(at, 900))
+    one = packed.cached_attention(q[None, :2], k[None], v[None], torch.tensor([n], dtype=I32, device=DEV))
+    seen(one[0], slice(0, 2))
