@@ -662,8 +662,9 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
  * [batch, new_len, heads, head_dim], caches [batch, capacity, kv_heads, head_dim] with strides (sequence, token,
  * head); lens [batch] device int32 = tokens of each sequence, the new ones included.  Query i sees rows
  * j < min(capacity, lens[b] - new_len + 1 + i): where lens passes the capacity the rows that did not fit are missing
- * and the window stays; none: zeros.  Rows from lens[b] on are never used, whatever they hold.  The key axis is split over workgroups where rows are few and joined in a second launch (workspace:
- * tagan_cached_attn_workspace bytes, a function of these arguments only).  Limits as tagan_packed_attn_fwd. */
+ * and the window stays; none: zeros.  Rows from lens[b] on are never used, whatever they hold.  The key axis is split
+ * over workgroups where rows are few and joined in a second launch (workspace: tagan_cached_attn_workspace bytes, a
+ * function of these arguments only).  Limits as tagan_packed_attn_fwd; capacity below 2^31 - 1024. */
 size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,
                                    int32_t head_dim);
 int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacity, int32_t heads, int32_t kv_heads,

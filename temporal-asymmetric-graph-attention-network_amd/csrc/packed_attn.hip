@@ -1500,7 +1500,8 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
                       int64_t o_head, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("cached_attn", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    TAGAN_REQUIRE(batch >= 0 && batch <= 0x7fffffff && new_len >= 0 && capacity >= 0 && capacity <= 0x7fffffff,
+    // a tile's end behind the last key is counted in 31 bits
+    TAGAN_REQUIRE(batch >= 0 && batch <= 0x7fffffff && new_len >= 0 && capacity >= 0 && capacity <= 0x7fffffff - 1024,
                   TAGAN_ERR_ARG, "cached_attn: batch %lld new_len %d capacity %lld", (long long)batch, new_len,
                   (long long)capacity);
     if (batch == 0 || new_len == 0) return TAGAN_OK;

@@ -355,7 +355,7 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     j < lens[b] - L + 1 + i of the cache, and zeros come back where that is none.  A length past the capacity leaves
     that window where it is (the rows that ``rotary_append`` had no room for are missing from it).  Rows from ``lens[b]``
     on are not used, whatever they hold.  The caches are read in place: unit feature stride, other strides and the start on 16 bytes, token strides
-    up to 2^21 elements (RuntimeError otherwise).  No autograd."""
+    up to 2^21 elements, fewer than 2^31 - 1024 rows (RuntimeError otherwise).  No autograd."""
     _storage(q, k_cache, v_cache)
     _cache(k_cache, "k_cache")
     _cache(v_cache, "v_cache")

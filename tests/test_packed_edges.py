@@ -147,3 +147,16 @@ def test_what_a_row_sees_reaches_it_whatever_its_weight(dtype, bad, d):
     seen(out, slice(at, 900))
     one = packed.cached_attention(q[None, :2], k[None], v[None], torch.tensor([n], dtype=I32, device=DEV))
     seen(one[0], slice(0, 2))
+
+
+# ----------------------------------------------------------------------------- C entries: refused before any launch
+A = 0x10000   # a pointer that is never followed
+
+
+def test_cached_entry_leaves_room_behind_the_last_key():
+    """A tile's end is counted in 31 bits: the capacity stays a tile and more below 2^31, as packed keys do."""
+    L = _lib.lib()
+    for cap, status in ((0x7fffffff, -1), (0x7fffffff - 1023, -1), (-1, -1)):
+        got = L.tagan_cached_attn(0, 1, 1, cap, 2, 1, 8, A, 16, 16, 8, A, 0, 8, 8, A, 0, 8, 8, A, 0.25, A, 16, 16, 8, A,
+                                  1 << 40, None)
+        assert got == status, cap
