@@ -1207,6 +1207,8 @@ __global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_b
 
 // ------------------------------------------------------------------------------------------------ launches
 constexpr int MAX_DIM = 128, MAX_GROUP = 512;
+constexpr int64_t MAX_TOKENS = 0x7fffffff - 1024;   // a tile's end behind the last one is counted in 31 bits
+constexpr int64_t MAX_ROWS = 1ll << 40;             // tokens times heads: 16 TB of the smallest; their bytes stay in 64 bits
 
 bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int es) {
     return !((uintptr_t)p & 15) && (a * es) % 16 == 0 && (b * es) % 16 == 0 && (c * es) % 16 == 0;
@@ -1369,6 +1371,7 @@ extern "C" {
 size_t tagan_packed_attn_fwd_workspace(int32_t n_seq, int64_t nq, int64_t nk, int32_t heads, int32_t kv_heads,
                                        int32_t head_dim) {
     if (kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
+    if (nq > MAX_TOKENS || nk > MAX_TOKENS || nq > MAX_ROWS / heads) return 0;   // the forward refuses them
     const int n = packed_splits(TAGAN_F32, n_seq, nq, nk, heads, kv_heads, padded_dim(head_dim));   // bf16 splits no more
     return n == 1 ? 0 : (size_t)n * (size_t)nq * (size_t)heads * (size_t)(padded_dim(head_dim) + 2) * 4;
 }
@@ -1380,9 +1383,9 @@ int tagan_packed_attn_fwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           float* lse, void* rest, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("packed_attn_fwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= MAX_TOKENS && nk <= MAX_TOKENS,
                   TAGAN_ERR_ARG, "packed_attn_fwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
-    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= MAX_TOKENS && nq <= MAX_ROWS / heads, TAGAN_ERR_UNSUPPORTED,
                   "packed_attn_fwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0) return TAGAN_OK;
@@ -1438,9 +1441,9 @@ int tagan_packed_attn_bwd(int dtype, int32_t n_seq, int64_t nq, int64_t nk, int3
                           int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("packed_attn_bwd", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= 0x7fffffff - 1024 && nk <= 0x7fffffff - 1024,
+    TAGAN_REQUIRE(n_seq >= 0 && nq >= 0 && nk >= 0 && nq <= MAX_TOKENS && nk <= MAX_TOKENS,
                   TAGAN_ERR_ARG, "packed_attn_bwd: %d sequences, %lld and %lld tokens", n_seq, (long long)nq, (long long)nk);
-    TAGAN_REQUIRE(nq * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
+    TAGAN_REQUIRE(nq * (heads / kv_heads) <= MAX_TOKENS && nq <= MAX_ROWS / heads, TAGAN_ERR_UNSUPPORTED,
                   "packed_attn_bwd: %lld tokens of %d heads",
                   (long long)nq, heads);
     if (nq == 0 && nk == 0) return TAGAN_OK;
@@ -1489,6 +1492,7 @@ size_t tagan_cached_attn_workspace(int64_t batch, int32_t new_len, int64_t capac
                                    int32_t head_dim) {
     if (batch <= 0 || new_len <= 0 || kv_heads < 1 || heads < kv_heads || head_dim < 1 || head_dim > MAX_DIM) return 0;
     const int64_t rows = (int64_t)new_len * (heads / kv_heads);
+    if (batch > 0x7fffffff || batch * new_len > MAX_ROWS / heads) return 0;      // cached_attn refuses them
     const int n = cache_splits(batch, rows, kv_heads, capacity);
     return n == 1 ? 0 : (size_t)n * (size_t)batch * (size_t)(kv_heads * rows) * (size_t)(padded_dim(head_dim) + 2) * 4;
 }
@@ -1500,13 +1504,12 @@ int tagan_cached_attn(int dtype, int64_t batch, int32_t new_len, int64_t capacit
                       int64_t o_head, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check_shape("cached_attn", dtype, heads, kv_heads, head_dim, scale);
     if (rc != TAGAN_OK) return rc;
-    // a tile's end behind the last key is counted in 31 bits
-    TAGAN_REQUIRE(batch >= 0 && batch <= 0x7fffffff && new_len >= 0 && capacity >= 0 && capacity <= 0x7fffffff - 1024,
+    TAGAN_REQUIRE(batch >= 0 && batch <= 0x7fffffff && new_len >= 0 && capacity >= 0 && capacity <= MAX_TOKENS,
                   TAGAN_ERR_ARG, "cached_attn: batch %lld new_len %d capacity %lld", (long long)batch, new_len,
                   (long long)capacity);
     if (batch == 0 || new_len == 0) return TAGAN_OK;
-    TAGAN_REQUIRE((int64_t)new_len * (heads / kv_heads) <= 0x7fffffff - 1024, TAGAN_ERR_UNSUPPORTED,
-                  "cached_attn: %d new tokens of %d heads", new_len, heads);
+    TAGAN_REQUIRE((int64_t)new_len * (heads / kv_heads) <= MAX_TOKENS && batch * new_len <= MAX_ROWS / heads,
+                  TAGAN_ERR_UNSUPPORTED, "cached_attn: %lld x %d new tokens of %d heads", (long long)batch, new_len, heads);
     TAGAN_REQUIRE(lens, TAGAN_ERR_ARG, "cached_attn: null lens");
     const int es = dtype == TAGAN_F32 ? 4 : 2;
     AttnArgs A = {};

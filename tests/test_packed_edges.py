@@ -160,3 +160,23 @@ def test_cached_entry_leaves_room_behind_the_last_key():
         got = L.tagan_cached_attn(0, 1, 1, cap, 2, 1, 8, A, 16, 16, 8, A, 0, 8, 8, A, 0, 8, 8, A, 0.25, A, 16, 16, 8, A,
                                   1 << 40, None)
         assert got == status, cap
+
+
+@pytest.mark.parametrize("nq, heads", [(1 << 31, 1 << 30), (1 << 62, 1 << 30), (1 << 30, 1 << 30), (1 << 40, 8)])
+def test_forward_workspace_of_impossible_sizes(nq, heads):
+    """Sizes that no call takes need no workspace; their products do not overflow into a division by zero."""
+    code = ("import sys; sys.path.insert(0, '.')\nfrom tagan_amd import _lib\n"
+            "print(_lib.lib().tagan_packed_attn_fwd_workspace(1, %d, (1 << 31) - 4096, %d, %d, 16))" % (nq, heads, heads))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "0", (r.returncode, r.stderr[-300:])
+
+
+def test_entries_refuse_impossible_sizes():
+    L, n = _lib.lib(), 1 << 30
+    assert L.tagan_packed_attn_fwd(0, 1, n, n, n, n, 16, A, 16, 0, A, 16, 0, A, 16, 0, A, A, 1, 0.25, A, 16, 0, None, None,
+                                   A, 1 << 60, None) == -2
+    assert L.tagan_packed_attn_bwd(0, 1, n, n, n, n, 16, A, 16, 0, A, 16, 0, A, 16, 0, A, A, 1, 0.25, A, 16, 0, A, None, A,
+                                   16, 0, A, 16, 0, A, 16, 0, A, 16, 0, A, 1 << 60, None) == -2
+    assert L.tagan_cached_attn(0, n, 1 << 12, 64, n, n, 16, A, 0, 16, 0, A, 0, 16, 0, A, 0, 16, 0, A, 0.25, A, 0, 16, 0, A,
+                               1 << 60, None) == -2
+    assert L.tagan_cached_attn_workspace(n, 1 << 12, 64, n, n, 16) == 0
