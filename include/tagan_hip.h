@@ -603,7 +603,8 @@ int tagan_narrow_linear_bwd(int64_t M, int32_t K, int32_t N, const float* x, int
  * pairs are features (i, i + rot/2), or (2i, 2i + 1) with interleaved; features from `rot` on pass unchanged.
  * Angles are formed in fp64 (far positions), the turn in fp32.  inverse turns back: the gradient of the turn.
  * q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] with token / head strides in elements and unit
- * feature stride (heads or kv_heads 0: that tensor is absent); outputs may be the inputs.  head_dim <= 256.
+ * feature stride (heads or kv_heads 0: that tensor is absent); outputs may be the inputs.  head_dim <= 256, up to 2^28
+ * heads.
  * positions [tokens] of tagan_pos_type; inv_freq [rot / 2] fp64.  No workspace.
  * ------------------------------------------------------------------------- */
 enum tagan_pos_type { TAGAN_POS_I32 = 0, TAGAN_POS_I64 = 1, TAGAN_POS_F32 = 2, TAGAN_POS_F64 = 3 };

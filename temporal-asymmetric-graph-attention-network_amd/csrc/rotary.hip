@@ -18,6 +18,7 @@ namespace {
 
 constexpr int RB = 256;            // threads of a block
 constexpr int ROT_MAX_DIM = 256;   // one item per thread in the scalar form
+constexpr int ROT_MAX_HEADS = 1 << 28;   // a block counts the heads of its tokens, and a step behind them, in 31 bits
 
 struct RotTensor {
     const void* in;
@@ -224,6 +225,8 @@ int check_dims(const char* what, int dtype, int32_t heads, int32_t kv_heads, int
     TAGAN_REQUIRE(dtype == TAGAN_F32 || dtype == TAGAN_BF16, TAGAN_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
     TAGAN_REQUIRE(heads >= 0 && kv_heads >= 0 && heads + kv_heads > 0, TAGAN_ERR_ARG, "%s: heads %d, %d", what, heads,
                   kv_heads);
+    TAGAN_REQUIRE(heads <= ROT_MAX_HEADS && kv_heads <= ROT_MAX_HEADS, TAGAN_ERR_UNSUPPORTED,
+                  "%s: heads %d, %d (up to %d)", what, heads, kv_heads, ROT_MAX_HEADS);
     TAGAN_REQUIRE(dim >= 1 && dim <= ROT_MAX_DIM, TAGAN_ERR_UNSUPPORTED, "%s: head_dim %d (1 to %d)", what, dim,
                   ROT_MAX_DIM);
     TAGAN_REQUIRE(rot >= 2 && rot <= dim && rot % 2 == 0, TAGAN_ERR_ARG, "%s: %d of %d features turned", what, rot,

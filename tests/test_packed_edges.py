@@ -180,3 +180,13 @@ def test_entries_refuse_impossible_sizes():
     assert L.tagan_cached_attn(0, n, 1 << 12, 64, n, n, 16, A, 0, 16, 0, A, 0, 16, 0, A, 0, 16, 0, A, 0.25, A, 0, 16, 0, A,
                                1 << 60, None) == -2
     assert L.tagan_cached_attn_workspace(n, 1 << 12, 64, n, n, 16) == 0
+
+
+@pytest.mark.parametrize("heads, kv", [((1 << 28) + 1, 1), (1, (1 << 28) + 1), (0x7fffffff, 0)])
+def test_rotary_entries_count_heads_in_31_bits(heads, kv):
+    """A block counts the heads of four tokens, and the steps behind the last, in 31 bits."""
+    L = _lib.lib()
+    assert L.tagan_rotary(0, 1, heads, kv, 2, 2, A, 2, 2, A, 2, 2, A, 0, A, 1.0, 0, 0, A, 2, 2, A, 2, 2, None) == -2
+    if kv:
+        assert L.tagan_rotary_append(0, 1, 1, heads, kv, 2, 2, A, 2, 2, 2, A, 2, 2, 2, A, 2, 2, 2, A, A, 1.0, 0, A, 2, 2,
+                                     2, A, 2, 2, 2, A, 2, 2, 2, 8, None) == -2
