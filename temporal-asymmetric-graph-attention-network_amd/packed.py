@@ -223,7 +223,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     to rows ``lens[b] + i`` of the caches [B, capacity, kv_heads, d] in place and returns the turned q, in one launch.
 
     ``lens`` [B] int32 counts the rows already there and is not advanced; rows that would lie outside the capacity are
-    not written.  No autograd."""
+    not written.  No autograd; a backward that kept rows of the caches raises after it, as after any write in place."""
     _storage(q, k, v, k_cache, v_cache)
     _cache(k_cache, "k_cache")
     _cache(v_cache, "v_cache")
@@ -250,6 +250,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
              *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], lens.data_ptr(),
              inv_freq.data_ptr(), scale, 1 if interleaved else 0, out.data_ptr(), L * heads * d, heads * d, d,
              k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[1])
+        torch.autograd.graph.increment_version((k_cache, v_cache))   # a backward that kept them has to notice
     return out
 
 

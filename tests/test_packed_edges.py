@@ -190,3 +190,20 @@ def test_rotary_entries_count_heads_in_31_bits(heads, kv):
     if kv:
         assert L.tagan_rotary_append(0, 1, 1, heads, kv, 2, 2, A, 2, 2, 2, A, 2, 2, 2, A, 2, 2, 2, A, A, 1.0, 0, A, 2, 2,
                                      2, A, 2, 2, 2, A, 2, 2, 2, 8, None) == -2
+
+
+# ----------------------------------------------------------------------------- caches and autograd
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_append_to_a_cache_that_a_backward_still_reads(which):
+    """The rows that attention kept for its backward were overwritten: it has to say so, not to use them."""
+    gen, cap, hq, hk, d = _gen(24), 8, 4, 2, 16
+    q = _randn(gen, 4, hq, d).to(DEV).requires_grad_(True)
+    caches = _dev(_randn(gen, 1, cap, hk, d), _randn(gen, 1, cap, hk, d))
+    kept = [c[0, :4] if i == which else c[0, :4].clone() for i, c in enumerate(caches)]
+    freq, _ = packed.rotary_frequencies(d, device=DEV)
+    out = packed.attention(q, *kept, torch.tensor([0, 4], dtype=I32, device=DEV))
+    new = _dev(*(_randn(gen, 1, 2, h, d) for h in (hq, hk, hk)))
+    packed.rotary_append(*new, *caches, torch.tensor([1], dtype=I32, device=DEV), freq)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
