@@ -238,6 +238,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     for c in (k_cache, v_cache):
         if 0 in c.stride() and any(n > 1 and s <= 0 for n, s in zip(c.shape, c.stride())):
             _refuse("a cache with shared rows cannot be written")
+    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
+        _refuse("one tensor cannot be both caches: k and v would be written to the same rows")
     lens = _index(lens, "lens", B)
     if not math.isfinite(scale):
         _refuse("scale %g", scale)

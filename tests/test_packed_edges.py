@@ -207,3 +207,14 @@ def test_append_to_a_cache_that_a_backward_still_reads(which):
     packed.rotary_append(*new, *caches, torch.tensor([1], dtype=I32, device=DEV), freq)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+def test_append_refuses_one_tensor_as_both_caches():
+    q, k, v = (torch.zeros(2, 1, h, 16) for h in (4, 2, 2))
+    c, both = torch.zeros(2, 8, 2, 16), torch.zeros(2, 8, 2, 2, 16)
+    freq, lens = torch.ones(8, dtype=torch.float64), torch.zeros(2, dtype=I32)
+    with pytest.raises(ValueError, match="one tensor"):
+        packed.rotary_append(q, k, v, c, c, lens, freq)
+    for pair in ((c, c.clone()), both.unbind(2)):          # accepted up to the device
+        with pytest.raises(RuntimeError, match="HIP device"):
+            packed.rotary_append(q, k, v, *pair, lens, freq)
