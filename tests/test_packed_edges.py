@@ -218,3 +218,90 @@ def test_append_refuses_one_tensor_as_both_caches():
     for pair in ((c, c.clone()), both.unbind(2)):          # accepted up to the device
         with pytest.raises(RuntimeError, match="HIP device"):
             packed.rotary_append(q, k, v, *pair, lens, freq)
+
+
+# ----------------------------------------------------------------------------- cached attention within a narrow bound
+CACHED = [(6, L, 333, [0, 1, 2, 64, 332, 333], *h) for L in (1, 3)
+          for h in ((1, 1, 8), (8, 2, 64), (8, 1, 128), (12, 4, 96))]
+CACHED += [(2, 1, 9000, [9000, 4001], 8, 2, 128), (1, 40, 700, [690], 8, 2, 64), (3, 5, 30, [2, 5, 30], 64, 1, 16),
+           (60, 1, 70, [(7 * i) % 71 for i in range(60)], 2, 1, 16)]
+
+
+def _cache_inputs(B, L, cap, hq, hk, d, sharp=1.0, dtype=torch.float32):
+    gen = _gen(25)
+    return (_randn(gen, B, L, hq, d) * sharp).to(dtype), *(_randn(gen, B, cap, hk, d, dtype=dtype) for _ in range(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B, L, cap, lens, hq, hk, d", CACHED)
+def test_cached_attention_in_32_bits(B, L, cap, lens, hq, hk, d):
+    q, kc, vc = _cache_inputs(B, L, cap, hq, hk, d)
+    got = packed.cached_attention(*_dev(q, kc, vc, torch.tensor(lens, dtype=I32)))
+    _within(got, *_cached_want(q, kc, vc, lens), "%d x %d on %s" % (B, L, lens[:6]))
+
+
+@pytest.mark.parametrize("B, L, cap, lens, hq, hk, d", CACHED)
+def test_the_bound_refuses_zeros_and_a_missing_key(B, L, cap, lens, hq, hk, d):
+    """For every history with a key (two, where one is left out): zeros, the newest key left out, a tenth of them."""
+    q, kc, vc = _cache_inputs(B, L, cap, hq, hk, d)
+    want, tol = _cached_want(q, kc, vc, lens)
+
+    def caught(got, least):
+        bad = ((got - want).abs() > tol).flatten(1).any(1)
+        assert all(bool(bad[b]) for b, n in enumerate(lens) if n >= least)
+    caught(torch.zeros_like(want), 1)
+    caught(_cached_want(q, kc, vc, [n - 1 for n in lens])[0], max(2, L))
+    late = [max(0, n - n // 10) for n in lens]
+    caught(_cached_want(q, kc, vc, late)[0], max(20, L))
+
+
+def _boundary_values(n, hk, d):
+    """Values at the ends of every run of 64 keys and at the last key only, all positive: each is a part of every sum."""
+    gen = _gen(26)
+    v = torch.zeros(n, hk, d)
+    at = sorted({j for m in range(0, n, 64) for j in (m - 1, m) if j >= 0} | {n - 1})
+    v[at] = _randn(gen, len(at), hk, d).abs() + 0.5
+    return v, at
+
+
+@pytest.mark.parametrize("n, hq, hk, d", [(9000, 8, 2, 128), (4001, 4, 1, 64)])
+def test_the_bound_refuses_any_key_at_a_boundary(n, hq, hk, d):
+    q, kc, _ = _cache_inputs(1, 1, n, hq, hk, d, 0.1)
+    v, at = _boundary_values(n, hk, d)
+    G = hq // hk
+    for h in range(hk):
+        o, tol, P = _rows(q[0, 0, h * G:(h + 1) * G], kc[0, :, h], v[:, h], torch.ones(G, n, dtype=torch.bool), d ** -0.5,
+                          torch.float32)
+        gone = P[:, at, None] * v[at, h].double()[None]         # what the result lacks without that key: [G, at, d]
+        assert bool((gone > tol[:, None]).any(2).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, hq, hk, d", [(9000, 8, 2, 128), (4001, 4, 1, 64)])
+def test_keys_at_every_boundary_of_a_split_count(n, hq, hk, d):
+    q, kc, _ = _cache_inputs(1, 1, n, hq, hk, d, 0.1)
+    v, _ = _boundary_values(n, hk, d)
+    want, tol = _cached_want(q, kc, v[None], [n])
+    got = packed.cached_attention(*_dev(q, kc, v[None], torch.tensor([n], dtype=I32)))
+    _within(got, want, tol, "cached")
+    offs = _dev(torch.tensor([0, 1], dtype=I32), torch.tensor([0, n], dtype=I32))
+    got = packed.attention(*_dev(q[0], kc[0], v), *offs)
+    _within(got, want[0], tol[0], "packed")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [1, 5])
+def test_serving_in_32_bits(step):
+    """Every step of three histories against the caches as they then are."""
+    gen, hq, hk, d, cap = _gen(27), 4, 2, 32, 64
+    kc, vc = (torch.full((3, cap, hk, d), math.nan, device=DEV) for _ in range(2))
+    lens = torch.tensor([0, 7, 19], dtype=I32, device=DEV)
+    for c in (kc, vc):
+        for b, n in enumerate(lens.tolist()):
+            c[b, :n] = _randn(gen, n, hk, d).to(DEV)
+    freq, _ = packed.rotary_frequencies(16, device=DEV)
+    for _ in range(40 // step):
+        qn = packed.rotary_append(*_dev(*(_randn(gen, 3, step, h, d) for h in (hq, hk, hk))), kc, vc, lens, freq)
+        lens += step
+        got = packed.cached_attention(qn, kc, vc, lens)
+        _within(got, *_cached_want(qn.cpu(), kc.cpu(), vc.cpu(), lens.tolist()), "lengths %s" % lens.tolist())
