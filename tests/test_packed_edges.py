@@ -305,3 +305,87 @@ def test_serving_in_32_bits(step):
         lens += step
         got = packed.cached_attention(qn, kc, vc, lens)
         _within(got, *_cached_want(qn.cpu(), kc.cpu(), vc.cpu(), lens.tolist()), "lengths %s" % lens.tolist())
+
+
+# ----------------------------------------------------------------------------- bf16: what the output's rounding took away
+# All scores are equal (q or k is zero), so the forward's probabilities are ones before the division and lose nothing as
+# bf16 operands.  Values are multiples of 1/2 near 64: a sum of 5000 stays below 2^23 halves and is exact in fp32, in any
+# order and in splits (their weights are ones too).  So out and its rest together are within 2^-16 (two roundings) and 8 W
+# (the division) of the mean.  With their large common part dP - rowsum(dO O) is a small difference of large terms, and
+# the output's own rounding (2^-8) would drown it; q, k and dO have a common part, so that
+# no sum over keys or rows averages it away.
+REST = [([3, 2, 4], [3, 2, 4], True), ([65], [65], True), ([90, 2], [90, 2], False), ([2, 1], [4000, 900], True),
+        ([150], [5000], False)]
+
+
+def _equal_scores(lens, klens, zero, hk=2, G=2, d=64):
+    gen = _gen(28)
+    n, nk = sum(lens), sum(klens)
+    q, k, do = (_randn(gen, m, h, d, dtype=torch.bfloat16) for m, h in ((n, hk * G), (nk, hk), (n, hk * G)))
+    v = ((_randn(gen, nk, hk, d) * 2).round() / 2 + 64).to(torch.bfloat16)
+    q, k, do = q + 1, k + 1, do + 1
+    (q if zero == "q" else k).zero_()
+    offs = [torch.tensor([0, *torch.tensor(x).cumsum(0).tolist()], dtype=I32) for x in (lens, klens)]
+    return q, k, v, do, *offs
+
+
+def _equal_want(q, k, v, do, offs, koffs, causal, lost=0.0):
+    """out, dq, dk and their bounds in 64 bits; `lost` 1 takes rowsum(dO O) from the rounded output (a planted mistake)."""
+    n, hq, d = q.shape
+    nk, hk = k.shape[:2]
+    G, scale, u = hq // hk, d ** -0.5, UNIT[torch.bfloat16]
+    o, to = (torch.zeros(n, hq, d, dtype=torch.float64) for _ in range(2))
+    dq, tq = torch.zeros_like(o), torch.zeros_like(o)
+    dk, tk = (torch.zeros(nk, hk, d, dtype=torch.float64) for _ in range(2))
+    Q, K, V, D = (t.double() for t in (q, k, v, do))
+    for a, b, ka, kb in zip(offs.tolist(), offs.tolist()[1:], koffs.tolist(), koffs.tolist()[1:]):
+        lq, lk = b - a, kb - ka
+        see = torch.ones(lq, lk, dtype=torch.bool)
+        if causal:
+            see = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + lk - lq
+        P = see.double() / see.sum(1, keepdim=True)
+        for h in range(hq):
+            x, y, z, g = Q[a:b, h], K[ka:kb, h // G], V[ka:kb, h // G], D[a:b, h]
+            oh = P @ z
+            toh = (2.0 ** -16 + 8 * W) * (P @ z.abs())
+            o[a:b, h], to[a:b, h] = oh, toh
+            dP = g @ z.T
+            kept = oh + lost * (oh.to(torch.bfloat16).double() - oh)
+            delta = (g * kept).sum(1, keepdim=True)
+            dS = P * (dP - delta)
+            dd = (g.abs() * toh).sum(1, keepdim=True) + (d + 4) * W * (g.abs() * oh.abs()).sum(1, keepdim=True)
+            # P again from the log-sum-exp: log2 of the count and exp2, a few W of up to 13
+            tS = P * ((d + 4) * W * (g.abs() @ z.abs().T) + dd + 4 * W * (dP.abs() + delta.abs())) + 32 * W * dS.abs()
+            tS = tS * (1 + u) + u * dS.abs()
+            dq[a:b, h] = dS @ y * scale
+            tq[a:b, h] = (tS @ y.abs() + (lk + 8) * W * (dS.abs() @ y.abs())) * scale * (1 + u) + u * dq[a:b, h].abs()
+            dk[ka:kb, h // G] += dS.T @ x * scale
+            tk[ka:kb, h // G] += (tS.T @ x.abs() + (lq * G + 8) * W * (dS.abs().T @ x.abs())) * scale * (1 + u)
+    return o, to, dq, tq, dk, tk + u * dk.abs()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens, klens, causal", REST)
+@pytest.mark.parametrize("zero", ["q", "k"])
+def test_the_rest_of_the_rounding_is_kept_and_used(lens, klens, causal, zero):
+    split = sum(klens) > 4000
+    assert (packed.lib().tagan_packed_attn_fwd_workspace(len(lens), sum(lens), sum(klens), 4, 2, 64) > 0) == split
+    q, k, v, do, offs, koffs = _equal_scores(lens, klens, zero)
+    leaves = [t.requires_grad_(True) for t in _dev(q, k, v)]
+    out = packed.attention(*leaves, *_dev(offs, koffs), causal=causal)
+    o, to, dq, tq, dk, tk = _equal_want(q, k, v, do, offs, koffs, causal)
+    assert torch.equal(out.grad_fn.saved_tensors[3], out)
+    rest = out.grad_fn.saved_tensors[5]
+    _within(out.detach().double() + rest.double(), o, to, "out and its rest")
+    grads = torch.autograd.grad(out, leaves, do.to(DEV))
+    _within(grads[0], dq, tq, "dq")
+    _within(grads[1], dk, tk, "dk")
+
+
+@pytest.mark.parametrize("lens, klens, causal", REST)
+def test_the_bound_refuses_a_rest_of_zeros(lens, klens, causal):
+    for zero, which in (("q", 2), ("k", 4)):
+        args = _equal_scores(lens, klens, zero)
+        want, lost = _equal_want(*args, causal), _equal_want(*args, causal, lost=1.0)
+        assert bool(((lost[which] - want[which]).abs() > want[which + 1]).any()), zero
+        assert bool(((want[0].to(torch.bfloat16).double() - want[0]).abs() > want[1]).any())
