@@ -24,16 +24,13 @@ namespace tagan {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 #define TAGAN_LDS(T, p) ((__attribute__((address_space(3))) T*)(p))
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LAZY = 8.f;
-
 
 // ------------------------------------------------------------------------------------------------ fragments
 template <typename T>
@@ -358,8 +355,8 @@ __device__ __forceinline__ Found find_seq(const int32_t* offs, int n_seq, int n,
 }
 
 // Heaviest tiles first.  With up to 62 sequences (and the two runs outside them) a lane keeps one of them, and every
-// block finds its own tile: the rank-th in falling order of work, by bisection on the work W.  `first` and `count` give
-// the tiles of the lane's sequence whose work is at least W, which are [first, first + count) in either order of work.
+// block finds its own tile: the rank-th in falling order of work, by bisection on the work W.  at_least(W) counts the tiles
+// of the lane's sequence whose work is at least W: its first ones, for no tile has more than the one before.
 // A long sequence whose tiles begin last costs the launch a fifth of its time (six histories of 1188 to 4096 tokens, dK
 // and dV: 782 us against 640); the 20 wave sums are a few per cent of a long block, so only launches of few blocks do it,
 // and the row kernels, whose blocks are shorter, lost 8 % by it.
@@ -377,11 +374,11 @@ __device__ __forceinline__ int wave_max_int(int x) {
 // most: no tile has more work
 template <class AtLeast>
 __device__ __forceinline__ bool ranked(int rank, int most, AtLeast at_least, int& seq, int& tile) {
-    int first, lo = 0, hi = most + 1;          // count(lo) > rank >= count(hi)
-    if (wave_sum_int(at_least(0, first)) <= rank) return false;
+    int lo = 0, hi = most + 1;                 // count(lo) > rank >= count(hi)
+    if (wave_sum_int(at_least(0)) <= rank) return false;
     int above = 0;
     while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2, n = wave_sum_int(at_least(mid, first));
+        const int mid = lo + (hi - lo) / 2, n = wave_sum_int(at_least(mid));
         if (n > rank) lo = mid;
         else {
             hi = mid;
@@ -389,8 +386,7 @@ __device__ __forceinline__ bool ranked(int rank, int most, AtLeast at_least, int
         }
     }
     // the tiles of work lo exactly: in order of the sequences, those of one in order of their numbers
-    int f_hi;
-    const int n_hi = at_least(hi, f_hi), n = at_least(lo, first) - n_hi;
+    const int n_hi = at_least(hi), n = at_least(lo) - n_hi;
     int before = n;                            // inclusive sum over the lanes
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -400,8 +396,7 @@ __device__ __forceinline__ bool ranked(int rank, int most, AtLeast at_least, int
     }
     const int left = rank - above;
     seq = __ffsll((long long)__ballot(before > left)) - 1;
-    const int own = first < f_hi || n_hi == 0 ? first : f_hi + n_hi;   // where the exact ones begin
-    tile = __shfl(own, seq, 64) + left - __shfl(before - n, seq, 64);
+    tile = __shfl(n_hi, seq, 64) + left - __shfl(before - n, seq, 64);
     seq = __builtin_amdgcn_readfirstlane(seq);
     tile = __builtin_amdgcn_readfirstlane(tile);
     return true;
@@ -953,8 +948,7 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
         }
         const int tiles = (slk + KEYS - 1) / KEYS, most = wave_max_int(slq);
         // tile t is seen by lq - max(0, t KEYS - past) tokens (all of them when not causal), 0 at least
-        const bool found = ranked(vt, most, [&](int w, int& first) {
-            first = 0;
+        const bool found = ranked(vt, most, [&](int w) {
             if (w <= 0) return tiles;
             if (slq < w) return 0;
             const int span = slk - w;          // lq - w + past
@@ -1274,10 +1268,11 @@ int run_bwd(const AttnArgs& A, hipStream_t s) {
     // at 128 features: one wave's registers fill a SIMD.
     if (A.nq * A.G + A.nk < (int64_t)128 * A.n_seq) return launch_bwd<T, D, 1, 1, 1>(A, s);
     if constexpr (sizeof(T) == 4 && D == 128) return launch_bwd<T, D, 4, 1, 2>(A, s);
-    else if ((A.nk / 128 + A.n_seq + 2) * A.kv_heads >= 4 * 256 && D * sizeof(T) < 256)
-        return launch_bwd<T, D, 4, 1, 2>(A, s);
-    else
+    else {
+        if constexpr (D * sizeof(T) < 256)
+            if ((A.nk / 128 + A.n_seq + 2) * A.kv_heads >= 4 * 256) return launch_bwd<T, D, 4, 1, 2>(A, s);
         return launch_bwd<T, D, 4, 2, 2>(A, s);
+    }
 }
 
 // Splits of the key axis where rows are few: enough one-wave blocks for 16 to a CU, and at least `least` keys of the longest
