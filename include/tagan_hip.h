@@ -631,9 +631,9 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  *   out = softmax(scale q kᵀ over the visible keys) v
  * causal: query i sees keys j <= i + Lk - Lq (the last query sees the last key), so every query i < Lq - Lk sees none;
  * a row without a visible key, or outside every sequence, gives zeros.
- * head_dim: multiples of 8 up to 128; heads / kv_heads <= 512; scale > 0.  Pointers and strides (elements) on 16
- * bytes, feature stride 1, token strides of head_dim to 2^21, tokens times heads / kv_heads below 2^31 and tokens times
- * heads up to 2^40.
+ * head_dim: multiples of 8 up to 128; heads / kv_heads <= 512; scale of 2^-126 to 2^127, and scale log2(e) q.k within
+ * fp32's range.  Pointers and strides (elements) on 16 bytes, feature stride 1, token strides of head_dim to 2^21, tokens
+ * times heads / kv_heads below 2^31 and tokens times heads up to 2^40.
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
  * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
  * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values

@@ -1215,7 +1215,8 @@ int check_shape(const char* what, int dtype, int64_t heads, int64_t kv_heads, in
                   (long long)kv_heads, MAX_GROUP);
     TAGAN_REQUIRE(dim >= 8 && dim <= MAX_DIM && dim % 8 == 0, TAGAN_ERR_UNSUPPORTED,
                   "%s: head_dim %d (a multiple of 8 up to %d)", what, dim, MAX_DIM);
-    TAGAN_REQUIRE(isfinite(scale) && scale > 0.f, TAGAN_ERR_ARG, "%s: scale has to be positive and finite", what);
+    // scale log2(e) has to be a finite fp32 number too
+    TAGAN_REQUIRE(scale >= 0x1p-126f && scale <= 0x1p127f, TAGAN_ERR_ARG, "%s: scale has to lie in 2^-126 to 2^127", what);
     return TAGAN_OK;
 }
 

@@ -308,8 +308,8 @@ def _dims(d: int, scale: Optional[float]) -> float:
     if d < 8 or d > MAX_HEAD_DIM or d % 8:
         _refuse("heads of %d features (a multiple of 8 up to %d)", d, MAX_HEAD_DIM)
     scale = d ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        _refuse("scale %g has to be positive and finite", scale)
+    if not 2.0 ** -126 <= scale <= 2.0 ** 127:
+        _refuse("scale %g has to lie in 2^-126 to 2^127", scale)
     return scale
 
 
@@ -320,7 +320,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
 
     ``offsets`` [B + 1] int32 on the device, ascending: history b has queries ``offsets[b]`` to ``offsets[b + 1]`` and
     keys by ``offsets_k`` (None: the same).  Query head h reads key head ``h // (heads / kv_heads)``.  ``causal`` lets
-    query i of Lq see keys j <= i + Lk - Lq: the last query sees the last key.  ``scale`` defaults to d^-0.5.
+    query i of Lq see keys j <= i + Lk - Lq: the last query sees the last key.  ``scale`` defaults to d^-0.5;
+    scale log2(e) q·k has to stay within fp32's range.
 
     Queries that see no key (an empty history, or Lq > Lk with ``causal``) and tokens outside every history (before
     the first offset, behind the last) give zeros and get zero gradients; offsets beyond the token count are taken as

@@ -389,3 +389,14 @@ def test_the_bound_refuses_a_rest_of_zeros(lens, klens, causal):
         want, lost = _equal_want(*args, causal), _equal_want(*args, causal, lost=1.0)
         assert bool(((lost[which] - want[which]).abs() > want[which + 1]).any()), zero
         assert bool(((want[0].to(torch.bfloat16).double() - want[0]).abs() > want[1]).any())
+
+
+@pytest.mark.parametrize("scale", [3e38, 1e39, 2.0 ** 127 * 1.0001, 1e-39, 1e-46])
+def test_scales_beyond_the_range_of_fp32_are_refused(scale):
+    q, k, offs = torch.zeros(6, 4, 16), torch.zeros(6, 2, 16), torch.tensor([0, 6], dtype=I32)
+    with pytest.raises(ValueError, match="scale"):
+        packed.attention(q, k, k, offs, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        packed.cached_attention(q[:, None], k[:, None], k[:, None], torch.ones(6, dtype=I32), scale=scale)
+    assert _lib.lib().tagan_packed_attn_fwd(0, 1, 6, 6, 4, 2, 16, A, 64, 16, A, 32, 16, A, 32, 16, A, A, 1, scale, A, 64, 16,
+                                            None, None, None, 0, None) == -1
