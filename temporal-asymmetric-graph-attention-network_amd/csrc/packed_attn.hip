@@ -407,6 +407,7 @@ template <int ROWS>
 __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
     if (A.offs_q == nullptr) {
         s.index = quot(vt, A.by_tiles);
+        if (TAGAN_DBAD(s.index >= 0 && s.index < A.n_seq, s.index, A.n_seq)) return false;   // history of a tile
         s.tile = vt - s.index * (int)A.by_tiles.d;
         s.lq = (int)A.nq;
         s.q0 = s.k0 = 0;
@@ -433,7 +434,8 @@ __device__ __forceinline__ bool locate(const AttnArgs& A, int vt, Seq& s) {
         }
     }
     s.past = s.lk - s.lq;
-    return true;
+    // the sequence that the search found
+    return !TAGAN_DBAD(s.q0 >= 0 && s.q0 + s.lq <= A.nq && s.k0 >= 0 && s.k0 + s.lk <= A.nk, s.q0, s.k0);
 }
 
 // The rows of a wave and what they see.  Counts of rows (tokens times the group) stay below 2^31.
@@ -641,6 +643,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
     if constexpr (SPLIT) {
         // unnormalised sums, and behind those of all rows the maxima (in powers of two) and totals; a row's splits together
         const int64_t at = (sq.index * A.nq + sq.q0 + R.token) * A.heads + hk * A.G + R.g;
+        if (TAGAN_DBAD(at < A.part_rows && split < A.splits, at, split)) return;   // place in the workspace
         float* p = A.part + (at * A.splits + split) * D;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -701,6 +704,7 @@ __global__ void __launch_bounds__(JT) k_attn_join(AttnArgs A) {
     __shared__ float4 sums[JW][8];
     const int64_t at = blockIdx.x / CH;
     const int ch = blockIdx.x % CH, s = threadIdx.x, wave = s >> 6, lane = s & 63;
+    if (TAGAN_DBAD(at < A.part_rows, at, A.part_rows)) return;   // row of the workspace
     float2 ml = make_float2(-INFINITY, 0.f);
     if (s < A.splits) ml = ((const float2*)(A.part + A.part_rows * A.splits * D))[at * A.splits + s];
     const bool some = ml.y != 0.f;             // a split without a visible key has no base
@@ -972,6 +976,7 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
         q0 = same ? k0 : edge(A.offs_q, A.n_seq, (int)A.nq, i);
         lq = same ? lk : max(0, edge(A.offs_q, A.n_seq, (int)A.nq, i + 1) - q0);
     }
+    if (TAGAN_DBAD(k0 >= 0 && k0 + lk <= nk && q0 >= 0 && q0 + lq <= A.nq, k0, q0)) return;   // what the search found
     const int G = A.G, past = lk - lq, key = key0 + wk * 32 + (lane & 31);
     const bool mine = key < lk;
     const uint32_t bytes = (uint32_t)A.dim * sizeof(T);
