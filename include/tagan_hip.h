@@ -636,9 +636,12 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * times heads / kv_heads below 2^31 and tokens times heads up to 2^40.
  * lse (nullable; the backward needs it): fp32 [nq, heads], log2 of the row's sum of 2^(scale log2(e) q.k), +inf where
  * no key is seen.  rest (nullable, TAGAN_BF16 only): bf16 [nq, heads, head_dim], what the rounding of out took away; with
- * it the backward's row sums of dout * out are as exact as in fp32 (without it they carry out's rounding).  Values
+ * it the backward's row sums of dout * out take out to 16 bits (without it they carry out's rounding, 8 bits).  Values
  * (infinities and NaN too) of keys that a row does not see never reach that row's output; an infinite or NaN value that
  * it sees makes that feature of its output infinite or NaN, however small the weight.
+ * TAGAN_BF16: probabilities and the gradients of scores are rounded to bf16 as operands of their second product, which
+ * brings errors to about 1.4 times one rounding of the result; where nk <= 64 n_seq (roundings of few terms do not average
+ * out) they are two bf16 operands each, and errors are those of one rounding.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
  * gradients.  workspaces: tagan_packed_attn_fwd_workspace (where few queries meet many keys the key axis is split over
  * workgroups and joined in a second launch; 0 otherwise; enough for either type) and tagan_packed_attn_bwd_workspace

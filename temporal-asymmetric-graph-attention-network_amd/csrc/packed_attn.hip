@@ -61,7 +61,8 @@ __device__ __forceinline__ void mma(f32x16& c, const Frag<float>& a, const Frag<
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
 }
 
-// eight accumulator registers as an operand (bf16: one rounding to nearest even of each probability or its gradient)
+// eight accumulator registers as an operand (bf16: one rounding to nearest even of each probability or its gradient; the
+// matrix cores take no wider operand at this rate, and over many keys the roundings average out)
 __device__ __forceinline__ void from_acc(Frag<uint16_t>& f, const f32x16& c, int at) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.u[j] = f2bf2(c[at + 2 * j], c[at + 2 * j + 1]);
@@ -69,6 +70,16 @@ __device__ __forceinline__ void from_acc(Frag<uint16_t>& f, const f32x16& c, int
 __device__ __forceinline__ void from_acc(Frag<float>& f, const f32x16& c, int at) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f.v[j] = c[at + j];
+}
+
+// and what that rounding took away, as a second operand
+__device__ __forceinline__ void rest_of(Frag<uint16_t>& f, const f32x16& c, int at) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float a = c[at + 2 * j], b = c[at + 2 * j + 1];
+        const uint32_t u = f2bf2(a, b);
+        f.u[j] = f2bf2(a - __uint_as_float(u << 16), b - __uint_as_float(u & 0xffff0000u));
+    }
 }
 
 __device__ __forceinline__ void load_frag(Frag<uint16_t>& f, const uint16_t* p) {
@@ -482,7 +493,8 @@ struct Shape {
 // Four waves share a tile: two waves lost 40 % to the tiles' traffic, eight gained nothing, a third stage lost 3 %.
 // STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
 // many more blocks of a CU hide each other's waits.
-template <typename T, int D, int WAVES, bool SPLIT, int STAGES>
+// FINE (bf16): each probability as two operands, its bf16 value and the rest, for batches of short histories (few_keys).
+template <typename T, int D, int WAVES, bool SPLIT, int STAGES, bool FINE = false>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3) k_attn_fwd(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
     typedef Tile<T, D> TL;
@@ -538,7 +550,8 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
         TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, vstep, valid, bytes, vlay);
     };
     const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
-        if (min(kt + KT, kend) > R.least && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
+        // FINE: in every tile, for the rest of a weight is zero or negative
+        if ((FINE || min(kt + KT, kend) > R.least) && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
         if (kt >= R.wave_most) return;
         f32x16 s[NB];
 #pragma unroll
@@ -596,13 +609,15 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                Frag<T> pf;
+                Frag<T> pf, pr;
                 from_acc(pf, s[b], 8 * x);
+                if constexpr (FINE) rest_of(pr, s[b], 8 * x);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> vf;
                     TL::cols(vf, vs, at, 32 * b + 16 * x, d);
                     mma(o[d], vf, pf);
+                    if constexpr (FINE) mma(o[d], vf, pr);
                 }
             }
     };
@@ -804,7 +819,7 @@ constexpr int dq_keys() {
 }
 
 // dQ: rows as in the forward.
-template <typename T, int D, int WAVES, int STAGES>
+template <typename T, int D, int WAVES, int STAGES, bool FINE>
 __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks, char* ks0, char* ks1, char* vs0,
                                         char* vs1) {
     constexpr int KT = dq_keys<T, D, WAVES>(), NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
@@ -881,13 +896,15 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                Frag<T> pf;
+                Frag<T> pf, pr;
                 from_acc(pf, s, 8 * x);
+                if constexpr (FINE) rest_of(pr, s, 8 * x);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> kf;
                     TL::cols(kf, ks, at, 32 * b + 16 * x, d);
                     mma(dq[d], kf, pf);
+                    if constexpr (FINE) mma(dq[d], kf, pr);
                 }
             }
         }
@@ -933,7 +950,7 @@ constexpr int dkv_rows() {          // rows of a tile: 32 to a row wave, and eno
     constexpr int LEAST = 1024 * WK * WR / Tile<T, D>::ROW;
     return 32 * WR > LEAST ? 32 * WR : LEAST;
 }
-template <typename T, int D, int WK, int WR, int STAGES>
+template <typename T, int D, int WK, int WR, int STAGES, bool FINE>
 __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0, char* gs0, char* qs1, char* gs1,
                                          char* st0, char* st1, char* vl) {
     typedef Tile<T, D> TL;
@@ -1088,16 +1105,22 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            Frag<T> pf, sf;
+            Frag<T> pf, sf, pr, sr;
             from_acc(pf, s, 8 * x);
             from_acc(sf, dp, 8 * x);
+            if constexpr (FINE) {
+                rest_of(pr, s, 8 * x);
+                rest_of(sr, dp, 8 * x);
+            }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 Frag<T> f;
                 TL::cols(f, gs, at, q + 16 * x, d);
                 mma(dv[d], f, pf);
+                if constexpr (FINE) mma(dv[d], f, pr);
                 TL::cols(f, qs, at, q + 16 * x, d);
                 mma(dk[d], f, sf);
+                if constexpr (FINE) mma(dk[d], f, sr);
             }
         }
     };
@@ -1192,7 +1215,7 @@ constexpr int bwd_waves() {
 // Six histories to 4096 tokens, 16 heads over 4, 128 features, bf16: 0.84 to 0.92 ms for seven products (two are made
 // twice so that no sum needs atomics), 0.75 to 0.82 PFLOP/s; apart they took 0.99.  1200 fp32 histories to 64 tokens, 8
 // heads of 16: 87 us, matrix pipe busy 43 %.
-template <typename T, int D, int WK, int WR, int STAGES>
+template <typename T, int D, int WK, int WR, int STAGES, bool FINE>
 __global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_bwd(AttnArgs A) {
     typedef Tile<T, D> TL;
     constexpr int WAVES = WK * WR, QT = dkv_rows<T, D, WK, WR>(), KT = dq_keys<T, D, WAVES>();
@@ -1200,8 +1223,8 @@ __global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_b
     __shared__ __align__(16) char qs0[TILE], gs0[TILE], qs1[SECOND], gs1[SECOND], st0[QT * 8], st1[QT * 8];
     __shared__ __align__(16) char vl[D == 128 ? 32 * WK * TL::ROW : 16];
     const int block = (int)blockIdx.x;
-    if (block < A.key_blocks) attn_dkv<T, D, WK, WR, STAGES>(A, block, qs0, gs0, qs1, gs1, st0, st1, vl);
-    else attn_dq<T, D, WAVES, STAGES>(A, block - A.key_blocks, (int)gridDim.x - A.key_blocks, qs0, qs1, gs0, gs1);
+    if (block < A.key_blocks) attn_dkv<T, D, WK, WR, STAGES, FINE>(A, block, qs0, gs0, qs1, gs1, st0, st1, vl);
+    else attn_dq<T, D, WAVES, STAGES, FINE>(A, block - A.key_blocks, (int)gridDim.x - A.key_blocks, qs0, qs1, gs0, gs1);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
@@ -1245,6 +1268,15 @@ int check_tensor(const char* what, const char* name, const void* p, Strides& s, 
 // with a tile of its own for the framework's 16 features, half the products of 32
 #define TAGAN_BY_DIM16(T, dim, F) ((dim) <= 16 ? F<T, 16> : TAGAN_BY_DIM(T, dim, F))
 
+// bf16, up to 64 keys to an average history: the FINE kernels, which take each probability and each gradient of a score as
+// two operands.  The roundings of few terms do not average out, and dP - rowsum(dO O) is a small difference that the
+// forward's probabilities enter.  Errors over that of one rounding of the result, out / dQ / dK / dV, one operand and two:
+// 240 histories of 1 to 4 tokens, 8 heads of 16: 1.08 / 1.51 / 1.51 / 1.21 and 1.00 each; single dQ and dK of the smallest
+// batches 2.3 and 1.00; at 100 keys one operand gives 1.20 / 1.45 / 1.44 / 1.36, at 300 1.25 / 1.45 / 1.44 / 1.38.  Times:
+// 1200 histories to 64 tokens, 8 heads of 16: forward 23 and 24 us, backward 64 and 66; 16 heads over 4 of 64: 58 and 61,
+// 238 and 253; 400 of 50 tokens, 32 heads over 4 of 128: 109 and 113, 410 and 454.
+bool few_keys(const AttnArgs& A) { return A.nk <= (int64_t)64 * A.n_seq; }
+
 // a launch counts its threads in 32 bits
 bool fits_grid(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads && blocks <= 0x7fffffff; }
 
@@ -1255,7 +1287,12 @@ int launch_bwd(AttnArgs A, hipStream_t s) {
     TAGAN_REQUIRE(fits_grid(keys + rows, 64 * WK * WR), TAGAN_ERR_UNSUPPORTED, "packed_attn_bwd: too many tiles");
     A.ranked = A.n_seq >= 2 && A.n_seq <= ORDERED && keys < 16 * 256;
     A.key_blocks = (int32_t)keys;
-    k_attn_bwd<T, D, WK, WR, STAGES><<<(unsigned)(keys + rows), 64 * WK * WR, 0, s>>>(A);
+    bool fine = false;
+    if constexpr (sizeof(T) == 2) {
+        fine = few_keys(A);
+        if (fine) k_attn_bwd<T, D, WK, WR, STAGES, true><<<(unsigned)(keys + rows), 64 * WK * WR, 0, s>>>(A);
+    }
+    if (!fine) k_attn_bwd<T, D, WK, WR, STAGES, false><<<(unsigned)(keys + rows), 64 * WK * WR, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("packed_attn_bwd");
     return TAGAN_OK;
 }
@@ -1337,6 +1374,13 @@ int run_fwd(const AttnArgs& A, hipStream_t s) {
     const bool one = A.nq * A.G < (int64_t)64 * A.n_seq;
     const int64_t blocks = packed_blocks(A.n_seq, A.nq, A.G, A.kv_heads);
     TAGAN_REQUIRE(fits_grid(blocks, one ? 64 : 256), TAGAN_ERR_UNSUPPORTED, "packed_attn_fwd: too many tiles");
+    if constexpr (sizeof(T) == 2)
+        if (few_keys(A)) {
+            if (one) k_attn_fwd<T, D, 1, false, 1, true><<<(unsigned)blocks, 64, 0, s>>>(A);
+            else k_attn_fwd<T, D, 4, false, 2, true><<<(unsigned)blocks, 256, 0, s>>>(A);
+            TAGAN_CHECK_LAUNCH("packed_attn_fwd");
+            return TAGAN_OK;
+        }
     if (one) k_attn_fwd<T, D, 1, false, 1><<<(unsigned)blocks, 64, 0, s>>>(A);
     else k_attn_fwd<T, D, 4, false, 2><<<(unsigned)blocks, 256, 0, s>>>(A);
     TAGAN_CHECK_LAUNCH("packed_attn_fwd");

@@ -400,3 +400,119 @@ def test_scales_beyond_the_range_of_fp32_are_refused(scale):
         packed.cached_attention(q[:, None], k[:, None], k[:, None], torch.ones(6, dtype=I32), scale=scale)
     assert _lib.lib().tagan_packed_attn_fwd(0, 1, 6, 6, 4, 2, 16, A, 64, 16, A, 32, 16, A, 32, 16, A, A, 1, scale, A, 64, 16,
                                             None, None, None, 0, None) == -1
+
+
+# ----------------------------------------------------------------------------- bf16: short histories
+# Up to 64 keys to an average history each probability and each dS enters as two bf16 operands (2^-16): out and its rest are
+# within (2^-16 + 2 e + (S + 8) W) P|V| + 2^-16 |o|, rowsum(dO O) is as exact, and the gradients have their own rounding (u)
+# and those terms only.  Values with a large common part show the forward's share: the probabilities' bf16 rounding alone
+# (2^-8 each) would move the mean, and with it every dP - rowsum(dO O) of the row; values without one show the backward's.
+FINE = [([1, 2, 3, 4] * 8, None, 2, 2, 16, True), ([5, 20, 40, 64], None, 2, 1, 64, True), ([16, 9, 30], None, 16, 2, 32, True),
+        ([50, 50], None, 2, 2, 128, False), ([3, 1, 0], [40, 9, 90], 4, 2, 96, True)]
+
+
+def _short(lens, klens, hq, hk, d, common):
+    gen, klens = _gen(29), klens or lens
+    assert sum(klens) <= 64 * len(klens)
+    q, k, do = (_randn(gen, sum(x), h, d, dtype=torch.bfloat16) for x, h in ((lens, hq), (klens, hk), (lens, hq)))
+    v = (_randn(gen, sum(klens), hk, d) + common).to(torch.bfloat16)
+    if common:                                           # so that no sum averages a row's error away
+        q, k, do = q / 2 + 0.5, k / 2 + 0.5, do + 1
+    return q, k, v, do, *(torch.tensor([0, *torch.tensor(x).cumsum(0).tolist()], dtype=I32) for x in (lens, klens))
+
+
+def _short_want(q, k, v, do, offs, koffs, causal, planted=None):
+    """out, dq, dk, dv and their bounds in 64 bits.  Planted: one bf16 operand for the forward's or the backward's."""
+    n, hq, d = q.shape
+    nk, hk = k.shape[:2]
+    G, scale, u, u2 = hq // hk, d ** -0.5, UNIT[torch.bfloat16], 2.0 ** -16
+    res = [torch.zeros(m, h, d, dtype=torch.float64) for m, h in ((n, hq),) * 4 + ((nk, hk),) * 4]
+    o, to, dq, tq, dk, tk, dv, tv = res
+    Q, K, V, D = (t.double() for t in (q, k, v, do))
+    for a, b, ka, kb in zip(offs.tolist(), offs.tolist()[1:], koffs.tolist(), koffs.tolist()[1:]):
+        lq, S = b - a, kb - ka
+        if lq == 0:
+            continue
+        see = torch.ones(lq, S, dtype=torch.bool)
+        if causal:
+            see = torch.arange(S)[None] <= torch.arange(lq)[:, None] + S - lq
+        for h in range(hq):
+            x, y, z, g = Q[a:b, h], K[ka:kb, h // G], V[ka:kb, h // G], D[a:b, h]
+            s = ((x @ y.T) * scale).masked_fill(~see, -math.inf)
+            w = torch.exp(s - s.amax(1, keepdim=True))
+            total = w.sum(1, keepdim=True)
+            P = w / total
+            e = ((d + 4) * W * (x.abs() @ y.abs().T) * scale + ((s - s.amax(1, keepdim=True)).abs() + 16) * W)
+            e = e.masked_fill(~see, 0.0).amax(1, keepdim=True)
+            oh = ((w.to(torch.bfloat16).double() if planted == "forward" else w) @ z) / total
+            toh = (u2 + 2 * e + (S + 8) * W) * (P @ z.abs()) + u2 * oh.abs()
+            o[a:b, h], to[a:b, h] = oh, toh
+            dP, delta = g @ z.T, (g * oh).sum(1, keepdim=True)
+            dS = P * (dP - delta)
+            dd = (g.abs() * toh).sum(1, keepdim=True) + (d + 4) * W * (g.abs() * oh.abs()).sum(1, keepdim=True)
+            tS = P * ((d + 4) * W * (g.abs() @ z.abs().T) + dd + 4 * W * (dP.abs() + delta.abs()))
+            tS = (tS + (2 * e + 32 * W) * dS.abs()) * (1 + u2) + u2 * dS.abs()
+            Pb = P
+            if planted == "backward":
+                dS, Pb = dS.to(torch.bfloat16).double(), P.to(torch.bfloat16).double()
+            dv[ka:kb, h // G] += Pb.T @ g
+            tv[ka:kb, h // G] += (u2 + 2 * e.amax() + 32 * W + (lq * G + 8) * W) * (P.T @ g.abs()) * (1 + u)
+            dq[a:b, h] = dS @ y * scale
+            tq[a:b, h] = (tS @ y.abs() + (S + 8) * W * (dS.abs() @ y.abs())) * scale * (1 + u) + u * dq[a:b, h].abs()
+            dk[ka:kb, h // G] += dS.T @ x * scale
+            tk[ka:kb, h // G] += (tS.T @ x.abs() + (lq * G + 8) * W * (dS.abs().T @ x.abs())) * scale * (1 + u)
+    tk += u * dk.abs()
+    tv += u * dv.abs()
+    return res
+
+
+def _over_one_rounding(got, want):
+    """The error's norm over that of rounding the exact result once.  N elements' own roundings leave it within 5 / sqrt(N)
+    of 1 (five deviations); independent roundings of the same size in every term of its sums bring it to sqrt(2)."""
+    return float((got.detach().cpu().double() - want).norm() / (want.to(torch.bfloat16).double() - want).norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("common", [0, 64])
+@pytest.mark.parametrize("lens, klens, hq, hk, d, causal", FINE)
+def test_short_histories_lose_nothing_to_the_operands(lens, klens, hq, hk, d, causal, common):
+    q, k, v, do, offs, koffs = _short(lens, klens, hq, hk, d, common)
+    leaves = [t.requires_grad_(True) for t in _dev(q, k, v)]
+    out = packed.attention(*leaves, *_dev(offs, koffs), causal=causal)
+    o, to, dq, tq, dk, tk, dv, tv = _short_want(q, k, v, do, offs, koffs, causal)
+    _within(out.detach().double() + out.grad_fn.saved_tensors[5].double(), o, to, "out and its rest")
+    grads = torch.autograd.grad(out, leaves, do.to(DEV))
+    _within(grads[0], dq, tq, "dq")
+    _within(grads[1], dk, tk, "dk")
+    _within(grads[2], dv, tv, "dv")
+    if common == 0:
+        assert q.numel() > 625 and k.numel() > 2500
+        assert _over_one_rounding(grads[0], dq) < 1.2 and _over_one_rounding(grads[1], dk) < 1.2
+        assert _over_one_rounding(grads[2], dv) < 1.1
+    assert torch.equal(packed.attention(*(t.detach() for t in leaves), *_dev(offs, koffs), causal=causal), out)
+
+
+@pytest.mark.parametrize("lens, klens, hq, hk, d, causal", FINE)
+def test_the_bound_refuses_rounded_operands(lens, klens, hq, hk, d, causal):
+    args = _short(lens, klens, hq, hk, d, 64)
+    want, got = _short_want(*args, causal), _short_want(*args, causal, planted="forward")
+    for which in (0, 2, 4):
+        assert bool(((got[which] - want[which]).abs() > want[which + 1]).any()), which
+    args = _short(lens, klens, hq, hk, d, 0)
+    want, got = _short_want(*args, causal), _short_want(*args, causal, planted="backward")
+    for which, least in ((2, 1.2), (4, 1.2), (6, 1.1)):
+        assert _over_one_rounding(got[which].to(torch.bfloat16), want[which]) > least, which
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+def test_short_histories_keep_infinities(causal):
+    """A visible infinity is that infinity, not NaN, though the second operand's weights are zeros and negative ones too."""
+    gen, n = _gen(30), 50
+    q, k, v = (_randn(gen, n, h, 16, dtype=torch.bfloat16) for h in (4, 2, 2))
+    v[7, :, 3], v[9, :, 5] = math.inf, -math.inf
+    out = packed.attention(*_dev(q, k, v, torch.tensor([0, 20, 50], dtype=I32)), causal=causal).cpu()
+    rows = slice(9, 20) if causal else slice(0, 20)
+    assert bool((out[rows, :, 3] == math.inf).all()) and bool((out[rows, :, 5] == -math.inf).all())
+    assert bool(torch.isfinite(out[20:]).all()) and bool(torch.isfinite(out[rows][..., [0, 1, 2, 4, *range(6, 16)]]).all())
+    assert not causal or bool(torch.isfinite(out[:7]).all())
