@@ -640,8 +640,8 @@ int tagan_rotary_append(int dtype, int64_t batch, int32_t new_len, int32_t heads
  * (infinities and NaN too) of keys that a row does not see never reach that row's output; an infinite or NaN value that
  * it sees makes that feature of its output infinite or NaN, however small the weight.
  * TAGAN_BF16: probabilities and the gradients of scores are rounded to bf16 as operands of their second product, which
- * brings errors to about 1.4 times one rounding of the result; where nk <= 64 n_seq (roundings of few terms do not average
- * out) they are two bf16 operands each, and errors are those of one rounding.
+ * brings errors to about 1.4 times one rounding of the result.  Where nk <= 64 n_seq, sequences of up to 128 keys take
+ * two bf16 operands each (roundings of few terms do not average out) and have the error of one rounding.
  * The backward sums the group's rows into dk / dv in a fixed order (no atomics); rows outside every sequence get zero
  * gradients.  workspaces: tagan_packed_attn_fwd_workspace (where few queries meet many keys the key axis is split over
  * workgroups and joined in a second launch; 0 otherwise; enough for either type) and tagan_packed_attn_bwd_workspace

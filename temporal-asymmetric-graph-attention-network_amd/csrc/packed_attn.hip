@@ -31,6 +31,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LAZY = 8.f;
+constexpr int SHORT = 128;   // keys of a history up to which the FINE kernels take two operands
 
 // ------------------------------------------------------------------------------------------------ fragments
 template <typename T>
@@ -493,7 +494,8 @@ struct Shape {
 // Four waves share a tile: two waves lost 40 % to the tiles' traffic, eight gained nothing, a third stage lost 3 %.
 // STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
 // many more blocks of a CU hide each other's waits.
-// FINE (bf16): each probability as two operands, its bf16 value and the rest, for batches of short histories (few_keys).
+// FINE (bf16, batches of short histories: few_keys): each probability of a short one as two operands, its bf16 value and
+// the rest.
 template <typename T, int D, int WAVES, bool SPLIT, int STAGES, bool FINE = false>
 __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3) k_attn_fwd(AttnArgs A) {
     constexpr int KT = Shape<T, D, WAVES>::KT, NB = KT / 32, NC = D / 16, ND = (D + 31) / 32, ROWS = 32 * WAVES;
@@ -542,6 +544,7 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, base = 0.f, l = 0.f;   // largest score of the base, that in powers of two, sum over it
 
+    const bool two = FINE && sq.lk <= SHORT;
     int wild_from = 0x7fffffff;                // first key of the tiles that were tamed
     const typename TL::At at = TL::at();
     const auto load = [&](char* kb, char* vb, int kt) __attribute__((always_inline)) {
@@ -550,8 +553,8 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
         TL::template fill<KT, WAVES>(vb, V + (int64_t)kt * A.vs.tok, vstep, valid, bytes, vlay);
     };
     const auto tile = [&](char* ks, char* vs, int kt) __attribute__((always_inline)) {
-        // FINE: in every tile, for the rest of a weight is zero or negative
-        if ((FINE || min(kt + KT, kend) > R.least) && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
+        // with two operands in every tile, for the rest of a weight is zero or negative
+        if ((two || min(kt + KT, kend) > R.least) && tame_tile<T, KT * TL::ROW, WAVES>(vs)) wild_from = min(wild_from, kt);
         if (kt >= R.wave_most) return;
         f32x16 s[NB];
 #pragma unroll
@@ -609,15 +612,23 @@ __global__ void __launch_bounds__(WAVES * 64, sizeof(T) == 4 && D == 128 ? 1 : 3
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                Frag<T> pf, pr;
+                Frag<T> pf;
                 from_acc(pf, s[b], 8 * x);
-                if constexpr (FINE) rest_of(pr, s[b], 8 * x);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> vf;
                     TL::cols(vf, vs, at, 32 * b + 16 * x, d);
                     mma(o[d], vf, pf);
-                    if constexpr (FINE) mma(o[d], vf, pr);
+                }
+                if constexpr (FINE) {
+                    if (!two) continue;
+                    rest_of(pf, s[b], 8 * x);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        Frag<T> vf;
+                        TL::cols(vf, vs, at, 32 * b + 16 * x, d);
+                        mma(o[d], vf, pf);
+                    }
                 }
             }
     };
@@ -830,6 +841,7 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
     if (!locate<ROWS>(A, quot(blocks, A.by_kv) - 1 - vt, sq)) return;
     const Rows R = rows_of<ROWS>(A, sq);
     const int kend = R.most;
+    const bool two = FINE && sq.lk <= SHORT;
     const int64_t head = hk * A.G + R.g, tok = sq.q0 + R.token;
     const T* Q = (const T*)A.q + tok * A.qs.tok + head * A.qs.head;
     const T* DO = (const T*)A.dout + tok * A.dos.tok + head * A.dos.head;
@@ -896,15 +908,23 @@ __device__ __forceinline__ void attn_dq(const AttnArgs& A, int block, int blocks
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                Frag<T> pf, pr;
+                Frag<T> pf;
                 from_acc(pf, s, 8 * x);
-                if constexpr (FINE) rest_of(pr, s, 8 * x);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     Frag<T> kf;
                     TL::cols(kf, ks, at, 32 * b + 16 * x, d);
                     mma(dq[d], kf, pf);
-                    if constexpr (FINE) mma(dq[d], kf, pr);
+                }
+                if constexpr (FINE) {
+                    if (!two) continue;
+                    rest_of(pf, s, 8 * x);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        Frag<T> kf;
+                        TL::cols(kf, ks, at, 32 * b + 16 * x, d);
+                        mma(dq[d], kf, pf);
+                    }
                 }
             }
         }
@@ -1105,22 +1125,29 @@ __device__ __forceinline__ void attn_dkv(const AttnArgs& A, int block, char* qs0
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            Frag<T> pf, sf, pr, sr;
+            Frag<T> pf, sf;
             from_acc(pf, s, 8 * x);
             from_acc(sf, dp, 8 * x);
-            if constexpr (FINE) {
-                rest_of(pr, s, 8 * x);
-                rest_of(sr, dp, 8 * x);
-            }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 Frag<T> f;
                 TL::cols(f, gs, at, q + 16 * x, d);
                 mma(dv[d], f, pf);
-                if constexpr (FINE) mma(dv[d], f, pr);
                 TL::cols(f, qs, at, q + 16 * x, d);
                 mma(dk[d], f, sf);
-                if constexpr (FINE) mma(dk[d], f, sr);
+            }
+            if constexpr (FINE) {
+                if (lk > SHORT) continue;
+                rest_of(pf, s, 8 * x);
+                rest_of(sf, dp, 8 * x);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    Frag<T> f;
+                    TL::cols(f, gs, at, q + 16 * x, d);
+                    mma(dv[d], f, pf);
+                    TL::cols(f, qs, at, q + 16 * x, d);
+                    mma(dk[d], f, sf);
+                }
             }
         }
     };
@@ -1269,12 +1296,14 @@ int check_tensor(const char* what, const char* name, const void* p, Strides& s, 
 #define TAGAN_BY_DIM16(T, dim, F) ((dim) <= 16 ? F<T, 16> : TAGAN_BY_DIM(T, dim, F))
 
 // bf16, up to 64 keys to an average history: the FINE kernels, which take each probability and each gradient of a score as
-// two operands.  The roundings of few terms do not average out, and dP - rowsum(dO O) is a small difference that the
-// forward's probabilities enter.  Errors over that of one rounding of the result, out / dQ / dK / dV, one operand and two:
-// 240 histories of 1 to 4 tokens, 8 heads of 16: 1.08 / 1.51 / 1.51 / 1.21 and 1.00 each; single dQ and dK of the smallest
-// batches 2.3 and 1.00; at 100 keys one operand gives 1.20 / 1.45 / 1.44 / 1.36, at 300 1.25 / 1.45 / 1.44 / 1.38.  Times:
-// 1200 histories to 64 tokens, 8 heads of 16: forward 23 and 24 us, backward 64 and 66; 16 heads over 4 of 64: 58 and 61,
-// 238 and 253; 400 of 50 tokens, 32 heads over 4 of 128: 109 and 113, 410 and 454.
+// two operands in histories of up to 128 keys (and as one in a longer one beside them).  The roundings of few terms do not
+// average out, and dP - rowsum(dO O) is a small difference that the forward's probabilities enter.  Errors over that of one
+// rounding of the result, out / dQ / dK / dV, one operand and two: 240 histories of 1 to 4 tokens, 8 heads of 16: 1.08 /
+// 1.51 / 1.51 / 1.21 and 1.00 each; single dQ and dK of the smallest batches 2.4 and 1.00; at 100 keys one operand gives
+// 1.20 / 1.45 / 1.44 / 1.36, at 300 1.25 / 1.45 / 1.44 / 1.38.  Times: 1200 histories to 64 tokens, 8 heads of 16: forward 23
+// and 25 us, backward 64 and 69; 16 heads over 4 of 64: 58 and 60, 239 and 258; 400 of 50 tokens, 32 heads over 4 of 128:
+// 110 and 113, 412 and 451.  The same choice in the kernels of long batches cost those 2 % (128 features, six histories to
+// 4096) to 14 % (16 features, 16 of 1000).
 bool few_keys(const AttnArgs& A) { return A.nk <= (int64_t)64 * A.n_seq; }
 
 // a launch counts its threads in 32 bits

@@ -9,11 +9,13 @@ head, and positions enter as turns of the query and key features.
 * ``rotary_append`` / ``cached_attention``   serving: write new tokens behind each cached history, attend to it
 
 fp32 or bf16 storage, fp32 statistics and sums.  In bf16 each probability, and each gradient of a score, is rounded to bf16
-as an operand of its second product: errors are about 1.4 times those of one rounding of the result.  Batches of up to 64
-keys to an average history, where such roundings do not average out, keep what the rounding took away as a second operand
-and have the error of one rounding.  Everything runs on the current HIP stream of the tensors' device,
-allocates from PyTorch's caching allocator only, never waits for the device and can be captured in a HIP graph; offsets
-and lengths stay on the device.  Wrong arguments raise TypeError / ValueError before anything is launched.
+as an operand of its second product: errors are about 1.4 times those of one rounding of the result.  Over few keys such
+roundings do not average out: in batches of up to 64 keys to an average history, those of up to 128 keys keep what the
+rounding took away as a second operand and have the error of one rounding.
+
+Everything runs on the current HIP stream of the tensors' device, allocates from PyTorch's caching allocator only, never
+waits for the device and can be captured in a HIP graph; offsets and lengths stay on the device.  Wrong arguments raise
+TypeError / ValueError, and what only the C entries know of RuntimeError, before anything is launched.
 
 A captured backward: capture forward and backward together (``graph_step.GraphedStep``) and let no eager graph of the
 same leaves live across the capture: such a graph keeps the leaves' gradient accumulation on the eager stream, which a

@@ -516,3 +516,14 @@ def test_short_histories_keep_infinities(causal):
     assert bool((out[rows, :, 3] == math.inf).all()) and bool((out[rows, :, 5] == -math.inf).all())
     assert bool(torch.isfinite(out[20:]).all()) and bool(torch.isfinite(out[rows][..., [0, 1, 2, 4, *range(6, 16)]]).all())
     assert not causal or bool(torch.isfinite(out[:7]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[700] + [1] * 20, [1] * 10 + [128, 129, 3], [127, 2, 0, 0, 0, 400] + [5] * 10], ids=str)
+@pytest.mark.parametrize("hq, hk, d", [(2, 2, 16), (4, 1, 128)])
+def test_a_long_history_among_short_ones(lens, hq, hk, d):
+    """The batch's average is short; each history goes by its own keys."""
+    from test_gpu_packed import _attend
+    assert sum(lens) <= 64 * len(lens)
+    _attend(lens, lens, hq, hk, d, torch.bfloat16)
+    _attend(lens, lens, hq, hk, d, torch.bfloat16, causal=False)
