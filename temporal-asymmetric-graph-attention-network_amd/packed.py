@@ -332,8 +332,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     the first offset, behind the last) give zeros and get zero gradients; offsets beyond the token count are taken as
     the token count.  What a query does not see, infinities and NaN included, does not reach its output; an infinity or
     NaN in a value that it sees makes that feature of its output infinite or NaN, however small the weight.  Gradients
-    flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.  There is
-    no second derivative (``create_graph`` raises).
+    flow to q, k and v (sums over the group for k and v), in a fixed order: the same inputs give the same bits.
+    An infinity or NaN in q, k, v or the output's gradient may reach any gradient of its history, and of no other.  There
+    is no second derivative (``create_graph`` raises).
     """
     _storage(q, k, v)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:

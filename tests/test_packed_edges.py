@@ -527,3 +527,25 @@ def test_a_long_history_among_short_ones(lens, hq, hk, d):
     assert sum(lens) <= 64 * len(lens)
     _attend(lens, lens, hq, hk, d, torch.bfloat16)
     _attend(lens, lens, hq, hk, d, torch.bfloat16, causal=False)
+
+
+# ----------------------------------------------------------------------------- infinities and gradients
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens, d", [([40, 30, 9], 16), ([300, 200, 77], 128), ([20, 5, 900], 64)])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+def test_gradients_of_other_histories_keep_their_bits(dtype, lens, d, which):
+    """NaN and infinities in one history reach gradients of that history only."""
+    gen, n = _gen(31), sum(lens)
+    t = {x: _randn(gen, n, h, d, dtype=dtype) for x, h in (("q", 4), ("k", 2), ("v", 2), ("dout", 4))}
+    offs = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=I32).to(DEV)
+
+    def grads():
+        leaves = [x.to(DEV).requires_grad_(True) for x in (t["q"], t["k"], t["v"])]
+        return torch.autograd.grad(packed.attention(*leaves, offs), leaves, t["dout"].to(DEV))
+    want = grads()
+    at = lens[0] + 3
+    t[which][at, :, 2], t[which][at + 1, :, 5] = math.nan, math.inf
+    others = [*range(lens[0]), *range(lens[0] + lens[1], n)]
+    for got, w in zip(grads(), want):
+        assert torch.equal(got[others], w[others])
