@@ -371,7 +371,8 @@ __device__ __forceinline__ Found find_seq(const int32_t* offs, int n_seq, int n,
 // of the lane's sequence whose work is at least W: its first ones, for no tile has more than the one before.
 // A long sequence whose tiles begin last costs the launch a fifth of its time (six histories of 1188 to 4096 tokens, dK
 // and dV: 782 us against 640); the 20 wave sums are a few per cent of a long block, so only launches of few blocks do it,
-// and the row kernels, whose blocks are shorter, lost 8 % by it.
+// and the row kernels, whose blocks are shorter, lost 8 % by it (13 prompts of 5 to 2500, longest last, first or in the
+// middle: 243, 253 and 247 us).
 constexpr int ORDERED = 62;
 __device__ __forceinline__ int wave_sum_int(int x) {
 #pragma unroll
@@ -489,7 +490,7 @@ struct Shape {
 
 // A wave has 32 rows, a block WAVES times as many, and a tile of KT keys at a time.  A tile of 32 keys of 128 features costs
 // a wave 16 matrix instructions of 32 cycles and about 75 vector ones, 16 of them exponentials: the two pipes are near
-// balance.  One sequence of 16384 tokens, 16 heads over 2, bf16: 1.01 to 1.10 ms with the card's temperature (1.0 to 1.09
+// balance.  One sequence of 16384 tokens, 16 heads over 2, bf16: 1.00 to 1.13 ms with the card's temperature (0.97 to 1.1
 // PFLOP/s; a library product of that size reaches 1.38), matrix pipe busy 52 % of the cycles at 1.9 GHz, no LDS conflicts.
 // Four waves share a tile: two waves lost 40 % to the tiles' traffic, eight gained nothing, a third stage lost 3 %.
 // STAGES 2: the next tile arrives while this one is multiplied; 1 (short sequences, one-wave blocks): half the LDS, and as
@@ -1241,7 +1242,7 @@ constexpr int bwd_waves() {
 // Both in one launch, the key blocks first: they are the longer ones, and the row blocks fill the CUs that they leave.
 // Six histories to 4096 tokens, 16 heads over 4, 128 features, bf16: 0.84 to 0.92 ms for seven products (two are made
 // twice so that no sum needs atomics), 0.75 to 0.82 PFLOP/s; apart they took 0.99.  1200 fp32 histories to 64 tokens, 8
-// heads of 16: 87 us, matrix pipe busy 43 %.
+// heads of 16: 89 us, matrix pipe busy 45 %.
 template <typename T, int D, int WK, int WR, int STAGES, bool FINE>
 __global__ void __launch_bounds__(WK* WR * 64, (bwd_waves<T, D, WK>())) k_attn_bwd(AttnArgs A) {
     typedef Tile<T, D> TL;
@@ -1365,7 +1366,7 @@ int cache_splits(int64_t batch, int64_t rows, int64_t kv_heads, int64_t capacity
 // Packed sequences: blocks by the rows of an average sequence, splits by its keys, at least 256 to each.  A block takes
 // about `key` ns to a key (measured); where that comes to 20 us the axis is split, into as many as write their sums in a
 // quarter of that time (written and read at 3 TB/s), 64 MB at most.  Unsplit and split, 128 features: 16 x 8 tokens on 8192
-// keys, bf16, 8 heads over 2: 330 and 41 us; one causal history of 4096, a head: bf16 102 and 29 us, fp32 538 and 70 us;
+// keys, bf16, 8 heads over 2: 330 and 38 us; one causal history of 4096, a head: bf16 102 and 31 us, fp32 538 and 68 us;
 // two of 1024, 8 heads, bf16, stay unsplit: 33 and 46 us.
 int64_t packed_blocks(int64_t n_seq, int64_t nq, int64_t G, int64_t kv_heads) {
     return (nq * G / (nq * G < 64 * n_seq ? 32 : 128) + n_seq + 2) * kv_heads;
