@@ -8,6 +8,7 @@ planted mistake (in the 64-bit reference).  Bounds, with W = 2^-24 and u half a 
            |do| <= (u' + 2 e + (S + 8 + 2 * 520) W) P|V| + u |o|, u' = u for bf16 (each probability is rounded), else 0
 """
 import math
+import os
 import subprocess
 import sys
 
@@ -165,9 +166,10 @@ def test_cached_entry_leaves_room_behind_the_last_key():
 @pytest.mark.parametrize("nq, heads", [(1 << 31, 1 << 30), (1 << 62, 1 << 30), (1 << 30, 1 << 30), (1 << 40, 8)])
 def test_forward_workspace_of_impossible_sizes(nq, heads):
     """Sizes that no call takes need no workspace; their products do not overflow into a division by zero."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     code = ("import sys; sys.path.insert(0, '.')\nfrom tagan_amd import _lib\n"
             "print(_lib.lib().tagan_packed_attn_fwd_workspace(1, %d, (1 << 31) - 4096, %d, %d, 16))" % (nq, heads, heads))
-    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=root)
     assert r.returncode == 0 and r.stdout.strip() == "0", (r.returncode, r.stderr[-300:])
 
 
